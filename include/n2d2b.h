@@ -56,7 +56,13 @@ typedef enum n2d2b_activation {
 } n2d2b_activation;
 
 typedef enum n2d2b_pooling { N2D2B_POOL_MAX = 0, N2D2B_POOL_AVERAGE = 1 } n2d2b_pooling;
-typedef enum n2d2b_dtype { N2D2B_I8 = 0, N2D2B_I32 = 1 } n2d2b_dtype;
+typedef enum n2d2b_dtype {
+    N2D2B_I8 = 0,
+    N2D2B_I32 = 1,
+    N2D2B_F32 = 2,  /* the floating-point types appear at the token operators only (end of this file) */
+    N2D2B_F16 = 3,
+    N2D2B_BF16 = 4
+} n2d2b_dtype;
 
 /*
  * Per-output-channel rescale: the payload of N2D2's Scaling value type (include/Scaling.hpp:45-427;
@@ -329,6 +335,118 @@ int n2d2b_first_conv_noalloc(int device, const void* d_input, int batch, int hei
 /* Test hook, n2d2b_net_selftest_wait_timeout for this entry point: a bounded wait runs out as if in a kernel of a call to
  * n2d2b_first_conv_noalloc on that device and stream; the next call returns N2D2B_ERR_TIMEOUT. */
 int n2d2b_first_conv_noalloc_selftest_wait_timeout(int device, unsigned limit_us, n2d2b_stream stream);
+
+/*
+ * Token operators: the layers of a language model served in 8-bit integers.  They have no counterpart in the reference.
+ *
+ * Where a cell's Scaling is fixed when the network is quantized, these take scales measured at run time: one for each token of
+ * an activation, one for each output channel of a weight, one for each page and head of a cache of keys and values.  A layer
+ * chains them: n2d2b_rmsnorm_quantize -> n2d2b_matmul_i8 (queries, keys and values) -> n2d2b_kv_append -> n2d2b_kv_attention.
+ *
+ * All of them
+ *   - take device buffers, on the given device (whichever is current; the caller's current device is left or put back), and
+ *     enqueue their work on `stream`, without waiting, allocating or copying: they can be captured into a graph and replayed,
+ *     and calls on several streams may overlap as long as none writes what another one reads or writes.  They use no
+ *     workspace.  The first call of a kind on a device loads its kernel;
+ *   - return N2D2B_ERR_INVALID for what they do not take, before any GPU work;
+ *   - read and write rows of the given strides (in elements; 0: rows lie side by side) and nothing between or behind them;
+ *   - make the same result from the same inputs, bit for bit, whatever ran beside them.
+ * Buffers of one call may not overlap except where it says so.  A code q under a scale s stands for q * s, q in [-127, 127].
+ * A scale comes of a largest magnitude a as a * (1 / 127); up to 2^-100 it is 0, and so are its codes.  A row or page that holds a
+ * value that is not finite gets a scale that is not finite or not a number, and its values read as not a number.
+ */
+
+/* Waits for `stream` and returns N2D2B_ERR_TIMEOUT if a kernel of these operators gave up on a bounded wait on this device since the last
+ * check (its output is then incomplete), N2D2B_ERR_CUDA if the stream failed, else 0; n2d2b_net_check's counterpart. */
+int n2d2b_token_check(int device, n2d2b_stream stream);
+/* Test hook, n2d2b_net_selftest_wait_timeout for these operators: the next n2d2b_token_check returns N2D2B_ERR_TIMEOUT. */
+int n2d2b_token_selftest_wait_timeout(int device, unsigned limit_us, n2d2b_stream stream);
+
+/* Root-mean-square norm with 8-bit output, a scale for each row:
+ *   h = x + residual, rounded to dtype (h = x without a residual); u = h * weight (32 bits)
+ *   step = max|u| * (1/127);  codes = round(u * (1/step));  scales = step / sqrt(mean(h^2) + eps)
+ * so codes * scales is h * weight / sqrt(mean(h^2) + eps) rounded to 255 levels.  The squares are summed in 32 bits: h^2 has to stay
+ * below 2^127. */
+typedef struct n2d2b_norm {
+    int32_t dtype;             /* of x, residual, total and weight: N2D2B_F32, N2D2B_F16 or N2D2B_BF16 */
+    int32_t rows, columns;
+    float eps;
+    const void* x;
+    const void* residual;      /* NULL: none */
+    void* total;               /* h; with a residual only.  May be x or residual itself (same stride) */
+    const void* weight;        /* columns entries; NULL: ones */
+    int8_t* codes;
+    float* scales;             /* rows entries */
+    int64_t x_stride, residual_stride, total_stride, codes_stride;
+} n2d2b_norm;
+int n2d2b_rmsnorm_quantize(int device, const n2d2b_norm* norm, n2d2b_stream stream);
+
+/* Matrix product of 8-bit codes with a scale for each token (row of a) and each output channel (row of w):
+ *   out[i][j] = (sum over k of a[i][k] * w[j][k]) * a_scales[i] * w_scales[j] + bias[j]
+ * The sum is exact in 32 bits (k up to 131071; codes may be -128 here); the products with the scales and the bias are taken in 32
+ * bits and rounded once to dtype.  Rows of a or w that do not start on 16 bytes (address or stride) take a slower kernel. */
+typedef struct n2d2b_matmul {
+    int32_t dtype;             /* of out: N2D2B_F32, N2D2B_F16 or N2D2B_BF16 */
+    int32_t m, n, k;           /* tokens, output channels, input channels */
+    const int8_t* a;           /* [m][k] */
+    const float* a_scales;
+    const int8_t* w;           /* [n][k], as n2d2b_net_add_fc takes it */
+    const float* w_scales;
+    const float* bias;         /* n entries; NULL: none */
+    void* out;                 /* [m][n] */
+    int64_t a_stride, w_stride, out_stride;
+} n2d2b_matmul;
+int n2d2b_matmul_i8(int device, const n2d2b_matmul* matmul, n2d2b_stream stream);
+
+/* A paged cache of keys and values in 8 bits, one scale for each page and head (of keys, and of values). */
+typedef struct n2d2b_kv_cache {
+    int32_t nb_pages, nb_heads;
+    int32_t page_tokens;       /* 16, 32, 64 or 128 */
+    int32_t head_size;         /* 64 or 128 */
+    int8_t* k;                 /* [page][head][token][head_size], starting on 16 bytes */
+    int8_t* v;
+    float* k_scales;           /* [page][head] */
+    float* v_scales;
+} n2d2b_kv_cache;
+/* The sequences of a call.  Sequence b holds `lengths[b]` tokens, the new ones of this call included; token t lies in page
+ * page_table[b][t / page_tokens] at place t % page_tokens.  Its new tokens are rows starts[b] .. starts[b + 1] - 1 of the call's tensors and
+ * the last of its tokens by position; rows behind the last sequence are neither read nor written.  An idle sequence has length 0.
+ * A call reads lengths, starts and page_table on the device and checks what it reads: rows beyond nb_tokens and new tokens beyond
+ * max_new do not exist for it; a page number outside the cache (or beyond the row of the table) holds nothing to append to, and
+ * makes the outputs of the queries that see it not a number. */
+typedef struct n2d2b_kv_batch {
+    int32_t nb_sequences;
+    int32_t pages_per_sequence;  /* entries of a row of page_table */
+    int32_t nb_tokens;           /* rows of the call's tensors */
+    int32_t max_new;             /* bound of a sequence's new tokens */
+    const int32_t* page_table;   /* [nb_sequences][pages_per_sequence] */
+    const int32_t* lengths;      /* nb_sequences entries */
+    const int32_t* starts;       /* nb_sequences + 1 entries; NULL: one new token for each sequence, row b for sequence b */
+} n2d2b_kv_batch;
+
+/* Writes the new tokens' keys and values, [row][nb_heads][head_size] in dtype (N2D2B_F16 or N2D2B_BF16) with `stride` elements from a row to the next, into
+ * the cache.  For each page and head that gains tokens: scale' = max(scale, max|new| * (1/127)), where the scale counts only if the page
+ * held earlier tokens of the sequence; their codes become round(q * (scale / scale')), the new ones round(x * (1 / scale')).  Places
+ * behind the sequence's end keep their bytes.  A page that gains tokens must belong to one sequence of the call alone (full
+ * pages may be shared); k and v start on 16 bytes and the stride is a multiple of 8. */
+int n2d2b_kv_append(int device, const n2d2b_kv_cache* cache, const n2d2b_kv_batch* batch, const void* k, const void* v, int dtype, int64_t stride,
+                    n2d2b_stream stream);
+
+/* Attention of the new tokens' queries over the cache (append the call's tokens first): for query head h, key head h / (nb_query_heads / nb_heads),
+ *   out = sum over visible j of softmax_j(scale * q . k_j) * v_j
+ * A query at position p (the last new token stands at lengths - 1) sees the tokens j < length, with `causal` only j <= p, and with a
+ * `window` > 0 (causal only) only j > p - window.  One that sees nothing gives zeros.  Scores, the softmax's sums and the output's sums are
+ * held in 32 bits; queries and probabilities enter the products in 16 bits (11 significant ones, on a scale of their own row). */
+typedef struct n2d2b_attention {
+    int32_t dtype;             /* of q and out: N2D2B_F16 or N2D2B_BF16 */
+    int32_t nb_query_heads;    /* a multiple of the cache's heads */
+    int32_t causal, window;
+    float scale;
+    const void* q;             /* [row][nb_query_heads][head_size], starting on 16 bytes */
+    void* out;
+    int64_t q_stride, out_stride; /* from a row to the next; multiples of 8 */
+} n2d2b_attention;
+int n2d2b_kv_attention(int device, const n2d2b_kv_cache* cache, const n2d2b_kv_batch* batch, const n2d2b_attention* attention, n2d2b_stream stream);
 
 #ifdef __cplusplus
 }

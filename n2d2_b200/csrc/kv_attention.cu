@@ -1,0 +1,534 @@
+// Attention over the paged 8-bit cache.
+//
+//   s_j = scale * sK(page of j) * (q . k_j),   out = (sum_j e^(s_j) sV(page of j) v_j) / (sum_j e^(s_j))      over visible j
+//
+// in one pass over the tokens, with the running maximum of t_j = s_j log2(e) + log2 sV(page of j): the values' scales ride in the
+// exponent, so that p_j = 2^(t_j - max) is at most 1 whatever the scales are and enters the second product in 16 bits; the softmax's sum
+// adds p_j / sV(page of j).
+//
+// kv_attention_rows_kernel: 16 rows (new token x query head of one key head) a tile, for few rows: bound by reading the cache.
+// Codes become 16-bit floats in registers (bytes spliced into 1024 + u, minus 1152: exact) on their way into mma.m16n8k16; the products'
+// inner indices are permuted so that a thread's operands are consecutive bytes of a token.  Every warp streams 32 tokens at a
+// time through a ring of its own by TMA and keeps its own maximum, sums and output; the tokens of a sequence are split over the
+// warps of a cluster of up to 16 blocks, whose parts are joined through distributed shared memory at the end, so nothing has to be kept in
+// memory between kernels.
+#include <cstdio>
+#include <cstring>
+#include "kv_common.cuh"
+
+namespace n2d2b {
+
+struct AttendArgs {
+    KvArgs c;
+    const void* q;
+    void* out;
+    long long q_stride, out_stride;
+    float scale_log2;      // scale * log2(e)
+    int group;             // query heads of a key head
+    int causal, window;
+    int log_page;
+    int* status;
+};
+
+__device__ __forceinline__ void mma_f16(float* d, const unsigned* a, unsigned b0, unsigned b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// (bytes 0, 1) and (bytes 2, 3) of four codes + 128 as halves 1024 + u
+__device__ __forceinline__ unsigned splice(unsigned w, unsigned sel)
+{
+    unsigned r;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(w), "r"(0x64646464u), "r"(sel));
+    return r;
+}
+__device__ __forceinline__ unsigned less_1152(unsigned h)
+{
+    const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half(0x6480)));
+    return *reinterpret_cast<const unsigned*>(&d);
+}
+__device__ __forceinline__ uint4 lds128(unsigned addr)
+{
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ uint2 lds64(unsigned addr)
+{
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ float exp2_approx(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ unsigned pack_half2(float a, float b)
+{
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const unsigned*>(&h);
+}
+__device__ __forceinline__ unsigned cluster_rank()
+{
+    unsigned r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ unsigned cluster_size()
+{
+    unsigned r;
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ unsigned map_to_rank(unsigned addr, unsigned rank)
+{
+    unsigned r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float ld_cluster(unsigned addr)
+{
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 ld_cluster4(unsigned addr)
+{
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+
+static constexpr int ROWS_WARPS = 4, ROWS_UNIT = 32, ROWS_STAGES = 3;
+template <int D> struct RowsSmem {
+    static constexpr int STAGE = 2 * ROWS_UNIT * D;                    // keys, then values
+    static constexpr int RING = ROWS_WARPS * ROWS_STAGES * STAGE;
+    static constexpr int PITCH = D + 4;                                // floats of a row of a part
+    static constexpr int PART = 16 * PITCH * 4;
+    static constexpr int BYTES = RING + 1024;                          // the parts take the ring's place
+    static_assert((ROWS_WARPS + 1) * PART + 4096 <= RING, "parts fit in the ring");
+};
+
+// One page's number and scales for a lane's unit half; what no query may see has no scale
+struct PageOf {
+    int number;
+    float k_scale, v_log, v_inverse;
+};
+__device__ __forceinline__ PageOf page_of(const KvArgs& c, int b, int head, int page, bool wanted)
+{
+    PageOf r = {0, 0.0f, 0.0f, 0.0f};
+    if (wanted) {
+        const float none = __int_as_float(0x7fffffff);
+        const int number = page < c.row ? c.table[(size_t)b * c.row + page] : -1;
+        if (number < 0 || number >= c.nb_pages) {
+            r.k_scale = none;
+        } else {
+            r.number = number;
+            r.k_scale = c.k_scales[(size_t)number * c.heads + head];
+            float v = c.v_scales[(size_t)number * c.heads + head];
+            if (v <= TOKEN_TINY) v = TOKEN_TINY;       // all codes are 0 then; any scale does
+            r.v_log = __log2f(v);
+            r.v_inverse = exp2_approx(-r.v_log);
+        }
+    }
+    return r;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(ROWS_WARPS * 32, 2) kv_attention_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                                                                               const AttendArgs a)
+{
+    typedef RowsSmem<D> S;
+    unsigned char* const smem = (unsigned char*)(((uintptr_t)dyn_smem() + 1023) & ~(uintptr_t)1023);
+    __shared__ __align__(8) unsigned long long full[ROWS_WARPS][ROWS_STAGES];
+    __shared__ int abort_flag;
+    pdl_launch_dependents();
+    if (threadIdx.x == 0) {
+        prefetch_tensor_map(&k_map);
+        prefetch_tensor_map(&v_map);
+        for (int i = 0; i < ROWS_WARPS * ROWS_STAGES; ++i) mbar_init(smem_u32(&full[0][0]) + 8 * i, 1);
+        abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    pdl_wait();
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c4 = lane & 3;
+    const int b = blockIdx.z, head = blockIdx.y % a.c.heads, tile = blockIdx.y / a.c.heads;
+    const unsigned rank = cluster_rank(), ranks = cluster_size();
+    const KvSequence s = kv_sequence(a.c, b);
+    const int rows = s.count * a.group - tile * 16;     // rows of the tile that exist
+    if (rows <= 0) return;                              // (the whole cluster)
+
+    // what the tile's rows see
+    const int t_first = tile * 16 / a.group, t_last = min(tile * 16 + 15, s.count * a.group - 1) / a.group;
+    int lo = 0, hi = s.length;
+    if (a.causal) {
+        hi = min(hi, s.begin + t_last + 1);
+        if (a.window) lo = max(0, s.begin + t_first + 1 - a.window);
+    }
+    const int capacity = a.c.row << a.log_page;         // tokens behind the row of the table are nowhere
+    hi = min(hi, capacity);
+    const int u_lo = lo / ROWS_UNIT, u_hi = hi > lo ? (hi + ROWS_UNIT - 1) / ROWS_UNIT : u_lo;
+    const int per_rank = (u_hi - u_lo + (int)ranks - 1) / (int)ranks;
+    const int u0 = u_lo + (int)rank * per_rank, u1 = min(u0 + per_rank, u_hi);
+
+    // a thread's rows are g and g + 8 of the tile
+    int pos[2];
+    float row_scale[2];
+    unsigned qa[D / 16][4];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        const int row = tile * 16 + g + 8 * r;
+        const bool there = g + 8 * r < rows;
+        const int t = row / a.group, h = row - t * a.group;
+        pos[r] = s.begin + t;
+        float v[D / 4];   // D / 4 consecutive values: D / 4 * c4 ...
+        unsigned top = 0;
+        const T* q = (const T*)a.q + (size_t)(s.first_row + t) * a.q_stride + (size_t)(head * a.group + h) * D + c4 * (D / 4);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (there) w = *reinterpret_cast<const uint4*>(q + 8 * i);
+            Elem<T>::unpack(w, v + 8 * i);
+        }
+#pragma unroll
+        for (int i = 0; i < D / 4; ++i) top = max(top, magnitude(v[i]));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // a power of two brings the row's largest value into [1, 4): exact, and a row of any size fits in halves
+        const int exponent = min((int)(top >> 23), 253);
+        const bool scaled = exponent > 0 && top < 0x7f800000u;
+        const float up = scaled ? __int_as_float((254 - exponent) << 23) : 1.0f;
+        row_scale[r] = a.scale_log2 * (scaled ? __int_as_float(exponent << 23) : 1.0f);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+            qa[k][r] = pack_half2(v[4 * k] * up, v[4 * k + 1] * up);
+            qa[k][r + 2] = pack_half2(v[4 * k + 2] * up, v[4 * k + 3] * up);
+        }
+    }
+
+    float acc[D / 8][4], top[2] = {-INFINITY, -INFINITY}, sum[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) sum[r] = (a.causal ? pos[r] : s.length - 1) >= capacity ? __int_as_float(0x7fffffff) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][e] = 0.0f;
+
+    // this warp's units: u0 + warp, + ROWS_WARPS, ...
+    const int mine = u1 - u0 > warp ? (u1 - u0 - warp + ROWS_WARPS - 1) / ROWS_WARPS : 0;
+    const unsigned ring = smem_u32(smem) + (unsigned)(warp * ROWS_STAGES * S::STAGE);
+    const unsigned bars = smem_u32(&full[warp][0]);
+    const bool small = a.log_page == 4;                 // a unit is two pages
+    PageOf held[2];
+    auto fetch_pages = [&](int from) {                  // lane i: pages of unit `from + i` of this warp
+        const int i = from + lane, token = (u0 + warp + i * ROWS_WARPS) * ROWS_UNIT;
+        held[0] = page_of(a.c, b, head, token >> a.log_page, i < mine);
+        held[1] = held[0];
+        if (small) held[1] = page_of(a.c, b, head, (token >> 4) + 1, i < mine && token + 16 < hi);
+    };
+    auto issue = [&](int i) {                           // unit i into its slot; every lane calls
+        const int n0 = __shfl_sync(0xffffffffu, held[0].number, i & 31), n1 = __shfl_sync(0xffffffffu, held[1].number, i & 31);
+        if (elect_one()) {
+            const unsigned bar = bars + 8u * (unsigned)(i % ROWS_STAGES), dst = ring + (unsigned)((i % ROWS_STAGES) * S::STAGE);
+            const int token = (u0 + warp + i * ROWS_WARPS) * ROWS_UNIT, page = 1 << a.log_page;
+            const int y0 = (n0 * a.c.heads + head) * page + (token & (page - 1));
+            mbar_expect_tx(bar, S::STAGE);
+            tma_load_2d(dst, &k_map, bar, 0, y0);
+            tma_load_2d(dst + ROWS_UNIT * D, &v_map, bar, 0, y0);
+            if (small) {
+                const int y1 = (n1 * a.c.heads + head) * page;
+                tma_load_2d(dst + 16 * D, &k_map, bar, 0, y1);
+                tma_load_2d(dst + ROWS_UNIT * D + 16 * D, &v_map, bar, 0, y1);
+            }
+        }
+        __syncwarp();
+    };
+
+    // offsets of a thread's operands inside a slot, as the copies swizzle them (rows of 128 bytes: chunk ^ row mod 8; of 64: chunk ^ (row / 2) mod 4)
+    unsigned k_off[2], v_off[2];
+    if (D == 128) {
+        k_off[0] = (unsigned)(g * 128 + (((2 * c4) ^ g) << 4));
+        k_off[1] = (unsigned)(g * 128 + (((2 * c4 + 1) ^ g) << 4));
+        v_off[0] = (unsigned)(2 * c4 * 128 + ((g ^ (2 * c4)) << 4));
+        v_off[1] = (unsigned)((2 * c4 + 1) * 128 + ((g ^ (2 * c4 + 1)) << 4));
+    } else {
+        k_off[0] = k_off[1] = (unsigned)(g * 64 + ((c4 ^ ((g >> 1) & 3)) << 4));
+        v_off[0] = (unsigned)(2 * c4 * 64 + (((g >> 1) ^ c4) << 4) + ((g & 1) << 3));
+        v_off[1] = v_off[0] + 64;
+    }
+
+    int issued = 0;
+    bool ok = true;
+    for (int i = 0; i < mine && ok; ++i) {
+        if ((i & 31) == 0) {                            // nothing of the next 32 units is under way yet
+            fetch_pages(i);
+            const int most = min(mine, i + ROWS_STAGES - 1);
+            for (; issued < most; ++issued) issue(issued);
+        }
+        // (the slot that unit i + STAGES - 1 takes was read in the iteration before)
+        if (issued < mine && issued < i + ROWS_STAGES && (issued >> 5) == (i >> 5)) { issue(issued); ++issued; }
+        const PageOf p0 = {0, __shfl_sync(0xffffffffu, held[0].k_scale, i & 31), __shfl_sync(0xffffffffu, held[0].v_log, i & 31), __shfl_sync(0xffffffffu, held[0].v_inverse, i & 31)};
+        const PageOf p1 = {0, __shfl_sync(0xffffffffu, held[1].k_scale, i & 31), __shfl_sync(0xffffffffu, held[1].v_log, i & 31), __shfl_sync(0xffffffffu, held[1].v_inverse, i & 31)};
+        const unsigned slot = ring + (unsigned)((i % ROWS_STAGES) * S::STAGE);
+        ok = mbar_wait_warp(bars + 8u * (unsigned)(i % ROWS_STAGES), (unsigned)(i / ROWS_STAGES) & 1u, &abort_flag, a.status, 21);
+        if (!ok) break;
+
+        float sc[4][4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[n][e] = 0.0f;
+            unsigned w[D / 16];
+            const unsigned at = slot + (unsigned)(n * 8 * D);
+#pragma unroll
+            for (int h = 0; h < D / 64; ++h) {
+                const uint4 x = lds128(at + k_off[h]);
+                w[4 * h] = x.x; w[4 * h + 1] = x.y; w[4 * h + 2] = x.z; w[4 * h + 3] = x.w;
+            }
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+                const unsigned u = w[k] ^ 0x80808080u;
+                mma_f16(sc[n], qa[k], less_1152(splice(u, 0x4140)), less_1152(splice(u, 0x4342)));
+            }
+        }
+        const int j0 = (u0 + warp + i * ROWS_WARPS) * ROWS_UNIT;
+        float best[2] = {top[0], top[1]};
+        const bool whole = j0 + ROWS_UNIT <= s.length && (!a.causal || (j0 + ROWS_UNIT - 1 <= s.begin + t_first && (!a.window || j0 > s.begin + t_last - a.window)));
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const PageOf& p = n < 2 ? p0 : p1;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = e >> 1, j = j0 + 8 * n + 2 * c4 + (e & 1);
+                float v = fmaf(sc[n][e], p.k_scale * row_scale[r], p.v_log);
+                if (!whole) {
+                    const bool seen = j < s.length && (!a.causal || (j <= pos[r] && (!a.window || j > pos[r] - a.window)));
+                    v = seen ? v : -INFINITY;
+                }
+                sc[n][e] = v;
+                best[r] = fmaxf(best[r], v);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            best[r] = fmaxf(best[r], __shfl_xor_sync(0xffffffffu, best[r], 1));
+            best[r] = fmaxf(best[r], __shfl_xor_sync(0xffffffffu, best[r], 2));
+        }
+        if (__any_sync(0xffffffffu, best[0] != top[0] || best[1] != top[1])) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float fade = best[r] == top[r] ? 1.0f : exp2_approx(top[r] - best[r]);
+                top[r] = best[r];
+                sum[r] *= fade;
+#pragma unroll
+                for (int d = 0; d < D / 8; ++d) { acc[d][2 * r] *= fade; acc[d][2 * r + 1] *= fade; }
+            }
+        }
+        const float base[2] = {top[0] == -INFINITY ? 0.0f : top[0], top[1] == -INFINITY ? 0.0f : top[1]};
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const float inv = n < 2 ? p0.v_inverse : p1.v_inverse;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float p = exp2_approx(sc[n][e] - base[e >> 1]);
+                sum[e >> 1] = fmaf(p, inv, sum[e >> 1]);
+                sc[n][e] = p;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const unsigned pa[4] = {pack_half2(sc[2 * k][0], sc[2 * k][1]), pack_half2(sc[2 * k][2], sc[2 * k][3]),
+                                    pack_half2(sc[2 * k + 1][0], sc[2 * k + 1][1]), pack_half2(sc[2 * k + 1][2], sc[2 * k + 1][3])};
+            const unsigned at = slot + (unsigned)(ROWS_UNIT * D + k * 16 * D);
+            unsigned x[4][D / 32];     // four tokens, D / 8 consecutive codes of each
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const unsigned from = at + v_off[t & 1] + (unsigned)((t >> 1) * 8 * D);
+                if (D == 128) {
+                    const uint4 y = lds128(from);
+                    x[t][0] = y.x; x[t][1] = y.y; x[t][D / 32 - 2] = y.z; x[t][D / 32 - 1] = y.w;
+                } else {
+                    const uint2 y = lds64(from);
+                    x[t][0] = y.x; x[t][1] = y.y;
+                }
+            }
+#pragma unroll
+            for (int w = 0; w < D / 32; ++w) {
+                // a word holds four codes of a token: pair them with the next token's
+                const unsigned a0 = x[0][w] ^ 0x80808080u, a1 = x[1][w] ^ 0x80808080u, b0 = x[2][w] ^ 0x80808080u, b1 = x[3][w] ^ 0x80808080u;
+                const unsigned al = __byte_perm(a0, a1, 0x5140), ah = __byte_perm(a0, a1, 0x7362);
+                const unsigned bl = __byte_perm(b0, b1, 0x5140), bh = __byte_perm(b0, b1, 0x7362);
+                mma_f16(acc[4 * w], pa, less_1152(splice(al, 0x4140)), less_1152(splice(bl, 0x4140)));
+                mma_f16(acc[4 * w + 1], pa, less_1152(splice(al, 0x4342)), less_1152(splice(bl, 0x4342)));
+                mma_f16(acc[4 * w + 2], pa, less_1152(splice(ah, 0x4140)), less_1152(splice(bh, 0x4140)));
+                mma_f16(acc[4 * w + 3], pa, less_1152(splice(ah, 0x4342)), less_1152(splice(bh, 0x4342)));
+            }
+        }
+        __syncwarp();
+    }
+    // copies under way (after a wait that gave up) land before the ring is given to the parts
+    if (!ok)
+        for (int i = 0; i < issued; ++i) mbar_wait_for(bars + 8u * (unsigned)(i % ROWS_STAGES), (unsigned)(i / ROWS_STAGES) & 1u, &abort_flag, a.status, 21, 1000000ull);
+
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
+        sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
+    }
+    __syncthreads();
+
+    // parts: [warp][row][D] and, behind them, maxima and sums; then the block's own part behind those
+    float* const parts = (float*)smem;
+    float* const part_top = parts + ROWS_WARPS * S::PART / 4;     // [warp][16], then sums
+    float* const part_sum = part_top + ROWS_WARPS * 16;
+    float* const own = part_sum + ROWS_WARPS * 16;                // [16][PITCH]
+    float* const own_top = own + S::PART / 4;
+    float* const own_sum = own_top + 16;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        float* const row = parts + (size_t)warp * (S::PART / 4) + (g + 8 * r) * S::PITCH + c4 * (D / 4);
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int d = 0; d < D / 8; d += 4)
+                *reinterpret_cast<float4*>(row + half * (D / 8) + d) =
+                    make_float4(acc[d][2 * r + half], acc[d + 1][2 * r + half], acc[d + 2][2 * r + half], acc[d + 3][2 * r + half]);
+        if (c4 == 0) {
+            part_top[warp * 16 + g + 8 * r] = top[r];
+            part_sum[warp * 16 + g + 8 * r] = sum[r];
+        }
+    }
+    __syncthreads();
+    const int there = min(rows, 16);
+    for (int i = threadIdx.x; i < there * (D / 4); i += ROWS_WARPS * 32) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        float m = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < ROWS_WARPS; ++w) m = fmaxf(m, part_top[w * 16 + r]);
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < ROWS_WARPS; ++w) {
+            const float t = part_top[w * 16 + r];
+            // a part that saw nothing but what is no number keeps it
+            const float f = t == m ? 1.0f : exp2_approx(t - m);
+            const float4 x = *reinterpret_cast<const float4*>(parts + (size_t)w * (S::PART / 4) + r * S::PITCH + d);
+            o.x = fmaf(x.x, f, o.x); o.y = fmaf(x.y, f, o.y); o.z = fmaf(x.z, f, o.z); o.w = fmaf(x.w, f, o.w);
+            l = fmaf(part_sum[w * 16 + r], f, l);
+        }
+        *reinterpret_cast<float4*>(own + r * S::PITCH + d) = o;
+        if (d == 0) { own_top[r] = m; own_sum[r] = l; }
+    }
+    if (ranks > 1) cluster_sync();
+    else __syncthreads();
+    // every block of the cluster finishes a share of the outputs
+    for (int i = (int)rank * ROWS_WARPS * 32 + (int)threadIdx.x; i < there * (D / 4); i += (int)ranks * ROWS_WARPS * 32) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        const unsigned at = smem_u32(own + r * S::PITCH + d), at_top = smem_u32(own_top + r), at_sum = smem_u32(own_sum + r);
+        float m = -INFINITY;
+        for (unsigned k = 0; k < ranks; ++k) m = fmaxf(m, ld_cluster(map_to_rank(at_top, k)));
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float l = 0.0f;
+        for (unsigned k = 0; k < ranks; ++k) {
+            const float t = ld_cluster(map_to_rank(at_top, k));
+            const float f = t == m ? 1.0f : exp2_approx(t - m);
+            const float4 x = ld_cluster4(map_to_rank(at, k));
+            o.x = fmaf(x.x, f, o.x); o.y = fmaf(x.y, f, o.y); o.z = fmaf(x.z, f, o.z); o.w = fmaf(x.w, f, o.w);
+            l = fmaf(ld_cluster(map_to_rank(at_sum, k)), f, l);
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const int row = tile * 16 + r, t = row / a.group, h = row - t * a.group;
+        T* const out = (T*)a.out + (size_t)(s.first_row + t) * a.out_stride + (size_t)(head * a.group + h) * D + d;
+        *reinterpret_cast<uint2*>(out) = make_uint2(Elem<T>::pack2(o.x * inv, o.y * inv), Elem<T>::pack2(o.z * inv, o.w * inv));
+    }
+    if (ranks > 1) cluster_sync();   // no block leaves while another reads its part
+}
+
+template <typename T, int D>
+static cudaError_t launch_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendArgs& a, int sequences, cudaStream_t s)
+{
+    static SmemLimitSet set, wide;
+    typedef RowsSmem<D> S;
+    cudaError_t e = raise_smem_limit(kv_attention_rows_kernel<T, D>, set, S::BYTES);
+    if (e != cudaSuccess) return e;
+    const long long tiles = ((long long)a.c.max_new * a.group + 15) / 16, blocks = tiles * a.c.heads * sequences;
+    const long long most = a.window ? min((long long)a.c.row << a.log_page, (long long)a.window + a.c.max_new) : (long long)a.c.row << a.log_page;
+    int split = 1;
+    // two blocks a multiprocessor; a block of a cluster has at least a unit for each of its warps
+    while (split < 16 && blocks * split * 2 <= 2 * token_sms() + blocks && (long long)split * ROWS_WARPS * ROWS_UNIT < most) split *= 2;
+    if (split > 8) {
+        int dev = 0;
+        cudaGetDevice(&dev);
+        const unsigned long long bit = dev >= 0 && dev < 64 ? 1ull << dev : 0ull;
+        if (!(wide.load(std::memory_order_relaxed) & bit)) {
+            e = cudaFuncSetAttribute(kv_attention_rows_kernel<T, D>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+            if (e != cudaSuccess) return e;
+            wide.fetch_or(bit, std::memory_order_relaxed);
+        }
+    }
+    if (tiles * a.c.heads > 65535) return cudaErrorInvalidConfiguration;
+    return launch_token(kv_attention_rows_kernel<T, D>, dim3((unsigned)split, (unsigned)(tiles * a.c.heads), (unsigned)sequences), ROWS_WARPS * 32, S::BYTES, split, s,
+                        k_map, v_map, a);
+}
+
+template <typename T>
+static cudaError_t launch_attention(const n2d2b_kv_cache& cache, const AttendArgs& a, int sequences, cudaStream_t s)
+{
+    CUtensorMap k_map, v_map;
+    const unsigned long long rows = (unsigned long long)cache.nb_pages * cache.nb_heads * cache.page_tokens;
+    const unsigned box = cache.page_tokens < ROWS_UNIT ? 16 : ROWS_UNIT;
+    const CUtensorMapSwizzle swizzle = cache.head_size == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+    if (!token_byte_map(&k_map, cache.k, cache.head_size, rows, cache.head_size, cache.head_size, box, swizzle)
+        || !token_byte_map(&v_map, cache.v, cache.head_size, rows, cache.head_size, cache.head_size, box, swizzle))
+        return cudaErrorInvalidValue;
+    return cache.head_size == 64 ? launch_rows<T, 64>(k_map, v_map, a, sequences, s) : launch_rows<T, 128>(k_map, v_map, a, sequences, s);
+}
+
+}  // namespace n2d2b
+
+extern "C" int n2d2b_kv_attention(int device, const n2d2b_kv_cache* cache, const n2d2b_kv_batch* batch, const n2d2b_attention* attention, n2d2b_stream stream)
+{
+    using namespace n2d2b;
+    AttendArgs a;
+    if (int rc = kv_check(cache, batch, a.c)) return rc;
+    if (!attention) return set_error(N2D2B_ERR_INVALID, "attention must not be NULL");
+    const n2d2b_attention& d = *attention;
+    if (d.dtype != N2D2B_F16 && d.dtype != N2D2B_BF16) return set_error(N2D2B_ERR_INVALID, "dtype must be N2D2B_F16 or N2D2B_BF16 (got %d)", d.dtype);
+    if (d.nb_query_heads < 1 || d.nb_query_heads % cache->nb_heads)
+        return set_error(N2D2B_ERR_INVALID, "nb_query_heads must be a multiple of the cache's %d heads (got %d)", cache->nb_heads, d.nb_query_heads);
+    if (d.window < 0 || (d.window > 0 && !d.causal)) return set_error(N2D2B_ERR_INVALID, "a window must not be negative and needs causal attention");
+    if (!(d.scale > -INFINITY && d.scale < INFINITY)) return set_error(N2D2B_ERR_INVALID, "scale must be finite");
+    if (batch->nb_sequences == 0 || batch->nb_tokens == 0 || a.c.max_new == 0) return 0;
+    if (!d.q || !d.out) return set_error(N2D2B_ERR_INVALID, "q and out must not be NULL");
+    const int64_t width = (int64_t)d.nb_query_heads * cache->head_size;
+    a.q_stride = d.q_stride ? d.q_stride : width;
+    a.out_stride = d.out_stride ? d.out_stride : width;
+    if (a.q_stride < width || a.q_stride % 8 || a.out_stride < width || a.out_stride % 8)
+        return set_error(N2D2B_ERR_INVALID, "strides must be 0 or multiples of 8 of at least %lld", (long long)width);
+    if (!token_aligned(d.q, 16) || !token_aligned(d.out, 16)) return set_error(N2D2B_ERR_INVALID, "q and out must start on 16 bytes");
+    a.group = d.nb_query_heads / cache->nb_heads;
+    if (((long long)a.c.max_new * a.group + 15) / 16 * cache->nb_heads > 65535)
+        return set_error(N2D2B_ERR_TOO_LARGE, "max_new x query heads exceeds %d rows", 65535 * 16);
+    a.q = d.q; a.out = d.out;
+    a.scale_log2 = d.scale * 1.4426950408889634f;
+    a.causal = d.causal ? 1 : 0;
+    a.window = (int64_t)d.window < (int64_t)batch->pages_per_sequence * cache->page_tokens ? d.window : 0;
+    a.log_page = cache->page_tokens == 16 ? 4 : cache->page_tokens == 32 ? 5 : cache->page_tokens == 64 ? 6 : 7;
+    const TokenDevice on(device);
+    if (on.err != cudaSuccess) return set_error(N2D2B_ERR_CUDA, "device %d is not usable: %s", device, cudaGetErrorString(on.err));
+    a.status = token_status_word();
+    if (!a.status) return set_error(N2D2B_ERR_CUDA, "the status word of the token operators has no address on device %d", device);
+    cudaError_t e;
+    if (d.dtype == N2D2B_F16) e = launch_attention<__half>(*cache, a, batch->nb_sequences, (cudaStream_t)stream);
+    else e = launch_attention<__nv_bfloat16>(*cache, a, batch->nb_sequences, (cudaStream_t)stream);
+    if (e != cudaSuccess) return set_error(N2D2B_ERR_CUDA, "attention launch failed: %s", cudaGetErrorString(e));
+    return 0;
+}

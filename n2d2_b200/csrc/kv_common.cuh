@@ -1,0 +1,66 @@
+// The paged cache as kernels see it, and the argument checks that appending to it and attending over it share.
+#pragma once
+#include "token_common.cuh"
+
+namespace n2d2b {
+
+struct KvArgs {
+    int8_t *k, *v;
+    float *k_scales, *v_scales;
+    const int *table, *lengths, *starts;
+    int nb_pages, heads, row;       // row: entries of a sequence's row of the page table
+    int nb_tokens, max_new;
+};
+
+// A sequence's part of the call, with what the device arrays say brought inside the call's bounds
+struct KvSequence {
+    int length;     // tokens it holds
+    int first_row;  // row of its first new token
+    int count;      // new tokens
+    int begin;      // position of the first of them; negative when there are more than the length holds
+};
+__device__ __forceinline__ KvSequence kv_sequence(const KvArgs& c, int b)
+{
+    KvSequence s;
+    s.length = max(c.lengths[b], 0);
+    int first = b, end = b + 1;
+    if (c.starts) { first = c.starts[b]; end = c.starts[b + 1]; }
+    first = min(max(first, 0), c.nb_tokens);
+    end = min(max(end, first), c.nb_tokens);
+    s.first_row = first;
+    s.count = min(end - first, c.max_new);
+    s.begin = s.length - s.count;
+    return s;
+}
+
+static inline int kv_check(const n2d2b_kv_cache* cache, const n2d2b_kv_batch* batch, KvArgs& a)
+{
+    if (!cache || !batch) return set_error(N2D2B_ERR_INVALID, "cache and batch must not be NULL");
+    if (cache->nb_pages < 1 || cache->nb_heads < 1)
+        return set_error(N2D2B_ERR_INVALID, "a cache has at least one page and one head (got %d, %d)", cache->nb_pages, cache->nb_heads);
+    if (cache->page_tokens != 16 && cache->page_tokens != 32 && cache->page_tokens != 64 && cache->page_tokens != 128)
+        return set_error(N2D2B_ERR_INVALID, "page_tokens must be 16, 32, 64 or 128 (got %d)", cache->page_tokens);
+    if (cache->head_size != 64 && cache->head_size != 128) return set_error(N2D2B_ERR_INVALID, "head_size must be 64 or 128 (got %d)", cache->head_size);
+    if ((long long)cache->nb_pages * cache->nb_heads > 2147483647ll / cache->page_tokens)
+        return set_error(N2D2B_ERR_TOO_LARGE, "pages x heads x page_tokens exceeds 2^31 - 1");
+    if (!cache->k || !cache->v || !cache->k_scales || !cache->v_scales) return set_error(N2D2B_ERR_INVALID, "the cache's buffers must not be NULL");
+    if (!token_aligned(cache->k, 16) || !token_aligned(cache->v, 16) || !token_aligned(cache->k_scales, 4) || !token_aligned(cache->v_scales, 4))
+        return set_error(N2D2B_ERR_INVALID, "the cache's codes must start on 16 bytes and its scales on 4");
+    if (batch->nb_sequences < 0 || batch->nb_tokens < 0 || batch->max_new < 0 || batch->pages_per_sequence < 1)
+        return set_error(N2D2B_ERR_INVALID, "invalid batch: %d sequences, %d tokens, at most %d new, %d pages a sequence", batch->nb_sequences,
+                         batch->nb_tokens, batch->max_new, batch->pages_per_sequence);
+    if (batch->nb_sequences > 32767) return set_error(N2D2B_ERR_TOO_LARGE, "nb_sequences = %d exceeds 32767", batch->nb_sequences);
+    if (batch->pages_per_sequence > 2147483647 / cache->page_tokens - 1)
+        return set_error(N2D2B_ERR_TOO_LARGE, "pages_per_sequence x page_tokens exceeds 2^31 - 1");
+    if (batch->nb_sequences > 0 && (!batch->page_table || !batch->lengths)) return set_error(N2D2B_ERR_INVALID, "page_table and lengths must not be NULL");
+    if (!token_aligned(batch->page_table, 4) || !token_aligned(batch->lengths, 4) || !token_aligned(batch->starts, 4))
+        return set_error(N2D2B_ERR_INVALID, "page_table, lengths and starts must start on 4 bytes");
+    a.k = cache->k; a.v = cache->v; a.k_scales = cache->k_scales; a.v_scales = cache->v_scales;
+    a.table = batch->page_table; a.lengths = batch->lengths; a.starts = batch->starts;
+    a.nb_pages = cache->nb_pages; a.heads = cache->nb_heads; a.row = batch->pages_per_sequence;
+    a.nb_tokens = batch->nb_tokens;
+    a.max_new = batch->starts ? batch->max_new : (batch->max_new < 1 ? batch->max_new : 1);
+    return 0;
+}
+
+}  // namespace n2d2b

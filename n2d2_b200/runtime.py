@@ -57,6 +57,38 @@ class TensorInfo(C.Structure):
         'channels', 'height', 'width', 'dtype', 'is_unsigned', 'producer', 'readable')]
 
 
+class Norm(C.Structure):
+    _fields_ = [('dtype', C.c_int32), ('rows', C.c_int32), ('columns', C.c_int32), ('eps', C.c_float), ('x', C.c_void_p), ('residual', C.c_void_p),
+                ('total', C.c_void_p), ('weight', C.c_void_p), ('codes', C.c_void_p), ('scales', C.c_void_p), ('x_stride', C.c_int64),
+                ('residual_stride', C.c_int64), ('total_stride', C.c_int64), ('codes_stride', C.c_int64)]
+
+
+class Matmul(C.Structure):
+    _fields_ = [('dtype', C.c_int32), ('m', C.c_int32), ('n', C.c_int32), ('k', C.c_int32), ('a', C.c_void_p), ('a_scales', C.c_void_p),
+                ('w', C.c_void_p), ('w_scales', C.c_void_p), ('bias', C.c_void_p), ('out', C.c_void_p), ('a_stride', C.c_int64),
+                ('w_stride', C.c_int64), ('out_stride', C.c_int64)]
+
+
+class KvCacheDesc(C.Structure):
+    _fields_ = [('nb_pages', C.c_int32), ('nb_heads', C.c_int32), ('page_tokens', C.c_int32), ('head_size', C.c_int32), ('k', C.c_void_p),
+                ('v', C.c_void_p), ('k_scales', C.c_void_p), ('v_scales', C.c_void_p)]
+
+
+class KvBatchDesc(C.Structure):
+    _fields_ = [('nb_sequences', C.c_int32), ('pages_per_sequence', C.c_int32), ('nb_tokens', C.c_int32), ('max_new', C.c_int32),
+                ('page_table', C.c_void_p), ('lengths', C.c_void_p), ('starts', C.c_void_p)]
+
+
+class Attention(C.Structure):
+    _fields_ = [('dtype', C.c_int32), ('nb_query_heads', C.c_int32), ('causal', C.c_int32), ('window', C.c_int32), ('scale', C.c_float),
+                ('q', C.c_void_p), ('out', C.c_void_p), ('q_stride', C.c_int64), ('out_stride', C.c_int64)]
+
+
+# floating-point types of the token operators
+F32, F16, BF16 = 2, 3, 4
+FLOAT_TYPES = {'f32': F32, 'f16': F16, 'bf16': BF16}
+
+
 _lib = None
 
 
@@ -109,6 +141,13 @@ def load():
                                                  C.POINTER(ConvDesc), C.c_void_p, C.c_void_p, C.POINTER(Quant),
                                                  C.c_void_p, C.c_void_p]
         lib.n2d2b_first_conv_noalloc_selftest_wait_timeout.argtypes = [C.c_int, C.c_uint, C.c_void_p]
+        lib.n2d2b_token_check.argtypes = [C.c_int, C.c_void_p]
+        lib.n2d2b_token_selftest_wait_timeout.argtypes = [C.c_int, C.c_uint, C.c_void_p]
+        lib.n2d2b_rmsnorm_quantize.argtypes = [C.c_int, C.POINTER(Norm), C.c_void_p]
+        lib.n2d2b_matmul_i8.argtypes = [C.c_int, C.POINTER(Matmul), C.c_void_p]
+        lib.n2d2b_kv_append.argtypes = [C.c_int, C.POINTER(KvCacheDesc), C.POINTER(KvBatchDesc), C.c_void_p, C.c_void_p, C.c_int, C.c_int64,
+                                        C.c_void_p]
+        lib.n2d2b_kv_attention.argtypes = [C.c_int, C.POINTER(KvCacheDesc), C.POINTER(KvBatchDesc), C.POINTER(Attention), C.c_void_p]
         _lib = lib
     return _lib
 
@@ -347,3 +386,63 @@ def first_conv_noalloc(d_in_ptr, batch, height, width, channels, in_unsigned, la
 
 def first_conv_noalloc_selftest_wait_timeout(limit_us=1000, device=0, stream=0):
     check(load().n2d2b_first_conv_noalloc_selftest_wait_timeout(device, limit_us, stream))
+
+
+# ---- token operators: layers of a language model served in 8-bit integers (raw device pointers, asynchronous on `stream`) ----
+
+def _float_type(dtype):
+    try:
+        return FLOAT_TYPES[dtype]
+    except KeyError:
+        raise ValueError(f'dtype must be one of {", ".join(FLOAT_TYPES)} (got {dtype!r})') from None
+
+
+def rmsnorm_quantize(x_ptr, rows, columns, weight_ptr, codes_ptr, scales_ptr, residual_ptr=None, total_ptr=None, dtype='bf16', eps=1e-6,
+                     x_stride=0, residual_stride=0, total_stride=0, codes_stride=0, device=0, stream=0):
+    """Root-mean-square norm of x (+ residual, the sum into total) as int8 codes with a scale for each row; see n2d2b_rmsnorm_quantize."""
+    d = Norm(_float_type(dtype), rows, columns, eps, x_ptr, residual_ptr, total_ptr, weight_ptr, codes_ptr, scales_ptr, x_stride,
+             residual_stride, total_stride, codes_stride)
+    check(load().n2d2b_rmsnorm_quantize(device, C.byref(d), stream))
+
+
+def matmul_i8(a_ptr, a_scales_ptr, w_ptr, w_scales_ptr, out_ptr, m, n, k, dtype='bf16', bias=None, a_stride=0, w_stride=0, out_stride=0,
+              device=0, stream=0):
+    """out = (a @ w.T) * a_scales[:, None] * w_scales + bias for int8 codes a [m][k], w [n][k]; see n2d2b_matmul_i8."""
+    d = Matmul(_float_type(dtype), m, n, k, a_ptr, a_scales_ptr, w_ptr, w_scales_ptr, bias, out_ptr, a_stride,
+               w_stride, out_stride)
+    check(load().n2d2b_matmul_i8(device, C.byref(d), stream))
+
+
+class KvBatch:
+    """The sequences of one step (an n2d2b_kv_batch): page table [nb_sequences][pages_per_sequence], lengths, rows of the new tokens.
+    Without `starts` every sequence has one new token."""
+
+    def __init__(self, nb_sequences, page_table_ptr, pages_per_sequence, lengths_ptr, nb_tokens, max_new, starts_ptr=None):
+        self.desc = KvBatchDesc(nb_sequences, pages_per_sequence, nb_tokens, max_new, page_table_ptr, lengths_ptr, starts_ptr)
+
+
+class KvCache:
+    """A paged cache of int8 keys and values, [nb_pages][nb_heads][page_tokens][head_size], with a float scale for each page and head
+    (an n2d2b_kv_cache).  The memory is the caller's."""
+
+    def __init__(self, k_ptr, v_ptr, k_scales_ptr, v_scales_ptr, nb_pages, nb_heads, page_tokens, head_size, device=0):
+        self.desc = KvCacheDesc(nb_pages, nb_heads, page_tokens, head_size, k_ptr, v_ptr, k_scales_ptr, v_scales_ptr)
+        self.device = device
+
+    def append(self, batch, k_ptr, v_ptr, stride=0, dtype='bf16', stream=0):
+        """Writes the new tokens' keys and values [row][nb_heads][head_size] into the cache; see n2d2b_kv_append."""
+        check(load().n2d2b_kv_append(self.device, C.byref(self.desc), C.byref(batch.desc), k_ptr, v_ptr, _float_type(dtype), stride, stream))
+
+    def attention(self, batch, q_ptr, out_ptr, nb_query_heads, scale, dtype='bf16', q_stride=0, out_stride=0, window=0, causal=True, stream=0):
+        """Attention of the new tokens' queries [row][nb_query_heads][head_size] over the cache; see n2d2b_kv_attention."""
+        d = Attention(_float_type(dtype), nb_query_heads, 1 if causal else 0, window, scale, q_ptr, out_ptr, q_stride, out_stride)
+        check(load().n2d2b_kv_attention(self.device, C.byref(self.desc), C.byref(batch.desc), C.byref(d), stream))
+
+
+def token_check(device=0, stream=0):
+    """Waits for `stream` and raises if a token operator's kernel gave up on a bounded wait."""
+    check(load().n2d2b_token_check(device, stream))
+
+
+def token_selftest_wait_timeout(limit_us=1000, device=0, stream=0):
+    check(load().n2d2b_token_selftest_wait_timeout(device, limit_us, stream))
