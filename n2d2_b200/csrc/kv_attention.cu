@@ -70,28 +70,6 @@ __device__ __forceinline__ unsigned pack_half2(float a, float b)
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const unsigned*>(&h);
 }
-__device__ __forceinline__ unsigned cluster_rank()
-{
-    unsigned r;
-    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ unsigned cluster_size()
-{
-    unsigned r;
-    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync()
-{
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ unsigned map_to_rank(unsigned addr, unsigned rank)
-{
-    unsigned r;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-    return r;
-}
 __device__ __forceinline__ float ld_cluster(unsigned addr)
 {
     float v;

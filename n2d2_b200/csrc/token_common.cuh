@@ -66,6 +66,30 @@ static inline cudaError_t launch_token(void (*kernel)(P...), dim3 grid, int thre
     return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
 }
 
+// ----------------------------------------------------------------------------- clusters
+__device__ __forceinline__ unsigned cluster_rank()
+{
+    unsigned r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ unsigned cluster_size()
+{
+    unsigned r;
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ unsigned map_to_rank(unsigned addr, unsigned rank)
+{
+    unsigned r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+
 // ----------------------------------------------------------------------------- element types
 template <typename T> struct Elem;
 template <> struct Elem<float> {

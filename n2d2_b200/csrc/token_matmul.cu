@@ -70,9 +70,365 @@ __global__ void __launch_bounds__(256) matmul_i8_any_kernel(const MatmulArgs p)
     }
 }
 
+// ----------------------------------------------------------------------------- tensor cores
+// Weights are the M operand of the MMAs (128 output channels to 128 TMEM lanes), tokens the N operand: a thread of the epilogue owns one output
+// channel (its scale and bias sit in registers), a warp stores 32 neighbouring channels of a token at a time, and a call of
+// few tokens has narrow tiles instead of empty rows.  A step of the ring is 128 bytes of k of every row, swizzled by TMA; rows and
+// bytes beyond the matrices read as zero.
+static constexpr int MM_K = 128, TILE_RING = 200 * 1024;
+
+// Scales, bias and store of `left` columns (tokens, at most 32) of a warp's 32 lanes (channels)
+template <typename T>
+__device__ __forceinline__ void store_columns(const MatmulArgs& p, const unsigned* acc, const float* sa, int token, int left, int channel, float sw, float bias)
+{
+    if (channel >= p.N) return;
+    T* out = (T*)p.out + (size_t)token * p.out_stride + channel;
+#pragma unroll
+    for (int c = 0; c < 32; ++c) {
+        if (c < left) *out = Elem<T>::from_float(fmaf((float)(int)acc[c] * sa[c], sw, bias));
+        out += p.out_stride;
+    }
+}
+
+// One tile of 128 channels x BN tokens a block.  Few tiles: the blocks of a cluster take parts of k and add their 32-bit sums up through
+// distributed shared memory, each finishing a share of the tile.  Warp 0 loads, warp 1 issues the MMAs, four warps store.
+template <typename T, int BN>
+__global__ void __launch_bounds__(192, 1) matmul_i8_tile_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap a_map, const MatmulArgs p,
+                                                                int stages, int* status)
+{
+    constexpr int STAGE = (128 + BN) * MM_K, COLUMNS = BN < 32 ? 32 : BN;
+    unsigned char* const smem = (unsigned char*)(((uintptr_t)dyn_smem() + 1023) & ~(uintptr_t)1023);
+    __shared__ __align__(8) unsigned long long full[12], empty[12], done;
+    __shared__ unsigned tmem_slot;
+    __shared__ int abort_flag;
+    __shared__ float sa[COLUMNS];
+    pdl_launch_dependents();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        prefetch_tensor_map(&w_map);
+        prefetch_tensor_map(&a_map);
+        for (int i = 0; i < stages; ++i) { mbar_init(smem_u32(&full[i]), 1); mbar_init(smem_u32(&empty[i]), 1); }
+        mbar_init(smem_u32(&done), 1);
+        abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"((unsigned)COLUMNS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const unsigned tmem = tmem_slot;
+    pdl_wait();
+
+    const unsigned rank = cluster_rank(), ranks = cluster_size();
+    const int n0 = blockIdx.y * 128, t0 = blockIdx.z * BN;
+    const int blocks = (p.K + MM_K - 1) / MM_K, per = (blocks + (int)ranks - 1) / (int)ranks;
+    const int from = (int)rank * per, count = max(0, min(per, blocks - from));
+    if (warp == 0) {
+        for (int i = 0; i < count; ++i) {
+            const int slot = i % stages;
+            if (i >= stages && !mbar_wait_issuer(smem_u32(&empty[slot]), (unsigned)(i / stages - 1) & 1u, &abort_flag, status, 31)) break;
+            if (elect_one()) {
+                const unsigned bar = smem_u32(&full[slot]), dst = smem_u32(smem) + (unsigned)(slot * STAGE);
+                mbar_expect_tx(bar, STAGE);
+                tma_load_2d(dst, &w_map, bar, (from + i) * MM_K, n0);
+                tma_load_2d(dst + 128 * MM_K, &a_map, bar, (from + i) * MM_K, t0);
+            }
+            __syncwarp();
+        }
+    } else if (warp == 1) {
+        const unsigned idesc = (2u << 4) | (1u << 7) | (1u << 10) | (((unsigned)BN >> 3) << 17) | ((128u >> 4) << 24);
+        const unsigned hi = (unsigned)(make_smem_desc(0u, 128) >> 32);
+        bool ok = true;
+        for (int i = 0; i < count && ok; ++i) {
+            const int slot = i % stages;
+            ok = mbar_wait_issuer(smem_u32(&full[slot]), (unsigned)(i / stages) & 1u, &abort_flag, status, 32);
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+                const unsigned w = ((smem_u32(smem) + (unsigned)(slot * STAGE)) & 0x3ffffu) >> 4, a = w + 128 * MM_K / 16;
+#pragma unroll
+                for (int k = 0; k < MM_K / 32; ++k) tc_mma_i8_lohi(tmem, w + 2 * k, a + 2 * k, hi, idesc, i > 0 || k > 0);
+                tc_commit(smem_u32(&empty[slot]));
+                if (i == count - 1) tc_commit(smem_u32(&done));
+            }
+            __syncwarp();
+        }
+    } else {
+        for (int i = (int)threadIdx.x - 64; i < BN; i += 128) sa[i] = t0 + i < p.M ? p.a_scales[t0 + i] : 0.0f;
+    }
+    __syncthreads();
+    const bool ok = count == 0 || mbar_wait_warp(smem_u32(&done), 0, &abort_flag, status, 33);
+    tc_fence_after();
+    if (!ok) __nanosleep(1000000);      // copies under way land before the block leaves
+    // the ring is free: every MMA has read its operands
+    int* const part = (int*)smem;       // [token][128 channels]
+    if (warp >= 2) {
+        const int quad = warp & 3, channel = quad * 32 + lane;
+        const float sw = ranks == 1 && n0 + channel < p.N ? p.w_scales[n0 + channel] : 0.0f;
+        const float bias = ranks == 1 && p.bias && n0 + channel < p.N ? p.bias[n0 + channel] : 0.0f;
+#pragma unroll 1
+        for (int c = 0; c < BN; c += 32) {
+            unsigned acc[32];
+            tc_ld32(tmem + ((unsigned)(quad * 32) << 16) + (unsigned)c, acc);
+            tc_wait_ld_into(acc);
+            if (ranks == 1) {
+                if (ok) store_columns<T>(p, acc, sa + c, t0 + c, min(BN - c, p.M - t0 - c), n0 + channel, sw, bias);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    if (c + i < BN) part[(c + i) * 128 + channel] = count ? (int)acc[i] : 0;
+            }
+        }
+    }
+    tc_fence_before();
+    if (ranks > 1) {
+        cluster_sync();
+        const int columns = min(BN, p.M - t0);
+        for (int i = (int)(rank * blockDim.x + threadIdx.x); i < columns * 32; i += (int)(ranks * blockDim.x)) {
+            const int c = i >> 5, channel = n0 + (i & 31) * 4;
+            int4 sum = make_int4(0, 0, 0, 0);
+            const unsigned at = smem_u32(part + i * 4);
+            for (unsigned r = 0; r < ranks; ++r) {
+                int4 v;
+                asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(map_to_rank(at, r)) : "memory");
+                sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+            }
+            const int s[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (channel + e < p.N)
+                    ((T*)p.out)[(size_t)(t0 + c) * p.out_stride + channel + e] =
+                        Elem<T>::from_float(fmaf((float)s[e] * sa[c], p.w_scales[channel + e], p.bias ? p.bias[channel + e] : 0.0f));
+        }
+        cluster_sync();     // no block leaves while another reads its sums
+    } else {
+        __syncthreads();
+    }
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((unsigned)COLUMNS) : "memory");
+    }
+}
+
+// ---- pairs of blocks on tiles of 256 x 256
+__device__ __forceinline__ void tma_load_2d_pair(unsigned dst, const CUtensorMap* tm, unsigned bar, int x, int y)
+{
+    // the barrier is the even block's of the pair, whichever block loads (bit 24 of a cluster address tells the two apart)
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(dst), "l"(tm), "r"(bar & 0xfeffffffu), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void tc_mma_i8_pair(unsigned d_tmem, unsigned a_lo, unsigned b_lo, unsigned desc_hi, unsigned idesc, unsigned accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "mov.b64 da, {%1, %3};\n\t"
+        "mov.b64 db, {%2, %3};\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], da, db, %4, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate) : "memory");
+}
+// arrives at the barrier of that address in both blocks of the pair
+__device__ __forceinline__ void tc_commit_pair(unsigned bar)
+{
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((unsigned short)3) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_even(unsigned bar)
+{
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(map_to_rank(bar, 0)) : "memory");
+}
+
+static constexpr int PAIR_STAGES = 6, PAIR_STAGE = 256 * MM_K, PAIR_SMEM = PAIR_STAGES * PAIR_STAGE + 1024, PAIR_THREADS = 320;
+
+// Persistent: a pair of blocks (one cta_group::2) walks over tiles of 256 channels x 256 tokens.  Each block holds its 128 channels and
+// half of the tokens of a step, so a byte is brought to a multiprocessor for twice the products of a single block's tile of 128 x 256; two
+// accumulators: the eight storing warps drain one while the next tile's MMAs fill the other.
+template <typename T>
+__global__ void __launch_bounds__(PAIR_THREADS, 1) matmul_i8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap a_map,
+                                                                         const MatmulArgs p, int tiles_n, int tiles, int* status)
+{
+    unsigned char* const smem = (unsigned char*)(((uintptr_t)dyn_smem() + 1023) & ~(uintptr_t)1023);
+    __shared__ __align__(8) unsigned long long full[PAIR_STAGES], empty[PAIR_STAGES], tfull[2], tempty[2];
+    __shared__ unsigned tmem_slot;
+    __shared__ int abort_flag;
+    pdl_launch_dependents();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const unsigned rank = cluster_rank();
+    if (threadIdx.x == 0) {
+        prefetch_tensor_map(&w_map);
+        prefetch_tensor_map(&a_map);
+        for (int i = 0; i < PAIR_STAGES; ++i) { mbar_init(smem_u32(&full[i]), 1); mbar_init(smem_u32(&empty[i]), 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&tfull[i]), 1); mbar_init(smem_u32(&tempty[i]), 16); }
+        abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after();
+    const unsigned tmem = tmem_slot;
+    pdl_wait();
+
+    const int blocks = (p.K + MM_K - 1) / MM_K;
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const int mine = pair < tiles ? (tiles - pair + pairs - 1) / pairs : 0;
+    if (warp == 0) {
+        bool ok = true;
+        int i = 0;
+        for (int t = 0; t < mine && ok; ++t) {
+            const int tile = pair + t * pairs, y_w = tile % tiles_n * 256 + (int)rank * 128, y_a = tile / tiles_n * 256 + (int)rank * 128;
+            for (int k = 0; k < blocks; ++k, ++i) {
+                const int slot = i % PAIR_STAGES;
+                if (i >= PAIR_STAGES && !mbar_wait_issuer(smem_u32(&empty[slot]), (unsigned)(i / PAIR_STAGES - 1) & 1u, &abort_flag, status, 34)) { ok = false; break; }
+                if (elect_one()) {
+                    const unsigned bar = smem_u32(&full[slot]), dst = smem_u32(smem) + (unsigned)(slot * PAIR_STAGE);
+                    if (rank == 0) mbar_expect_tx(bar, 2 * PAIR_STAGE);
+                    tma_load_2d_pair(dst, &w_map, bar, k * MM_K, y_w);
+                    tma_load_2d_pair(dst + 128 * MM_K, &a_map, bar, k * MM_K, y_a);
+                }
+                __syncwarp();
+            }
+        }
+        if (!ok) __nanosleep(1000000);      // copies under way land before the block leaves
+    } else if (warp == 1 && rank == 0) {
+        const unsigned idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
+        const unsigned hi = (unsigned)(make_smem_desc(0u, 128) >> 32);
+        bool ok = true;
+        int i = 0;
+        for (int t = 0; t < mine && ok; ++t) {
+            const unsigned d = tmem + (unsigned)((t & 1) * 256);
+            if (t >= 2 && !mbar_wait_issuer(smem_u32(&tempty[t & 1]), (unsigned)(t / 2 - 1) & 1u, &abort_flag, status, 35)) break;
+            tc_fence_after();
+            for (int k = 0; k < blocks; ++k, ++i) {
+                const int slot = i % PAIR_STAGES;
+                if (!mbar_wait_issuer(smem_u32(&full[slot]), (unsigned)(i / PAIR_STAGES) & 1u, &abort_flag, status, 36)) { ok = false; break; }
+                tc_fence_after();
+                if (elect_one()) {
+                    const unsigned w = ((smem_u32(smem) + (unsigned)(slot * PAIR_STAGE)) & 0x3ffffu) >> 4, a = w + 128 * MM_K / 16;
+#pragma unroll
+                    for (int q = 0; q < MM_K / 32; ++q) tc_mma_i8_pair(d, w + 2 * q, a + 2 * q, hi, idesc, k > 0 || q > 0);
+                    tc_commit_pair(smem_u32(&empty[slot]));
+                    if (k == blocks - 1) tc_commit_pair(smem_u32(&tfull[t & 1]));
+                }
+                __syncwarp();
+            }
+        }
+    } else if (warp >= 2) {
+        const int quad = warp & 3, half = (warp - 2) >> 2;
+        for (int t = 0; t < mine; ++t) {
+            const int tile = pair + t * pairs, channel = tile % tiles_n * 256 + (int)rank * 128 + quad * 32 + lane, t0 = tile / tiles_n * 256 + half * 128;
+            const float sw = channel < p.N ? p.w_scales[channel] : 0.0f, bias = p.bias && channel < p.N ? p.bias[channel] : 0.0f;
+            if (!mbar_wait_warp(smem_u32(&tfull[t & 1]), (unsigned)(t / 2) & 1u, &abort_flag, status, 37)) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < 128; c += 32) {
+                if (t0 + c >= p.M) break;
+                const float mine_sa = t0 + c + lane < p.M ? p.a_scales[t0 + c + lane] : 0.0f;
+                unsigned acc[32];
+                tc_ld32(tmem + ((unsigned)(quad * 32) << 16) + (unsigned)((t & 1) * 256 + half * 128 + c), acc);
+                tc_wait_ld_into(acc);
+                float sa[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) sa[i] = __shfl_sync(0xffffffffu, mine_sa, i);
+                store_columns<T>(p, acc, sa, t0 + c, p.M - t0 - c, channel, sw, bias);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_even(smem_u32(&tempty[t & 1]));
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();         // neither block leaves while the other's MMAs or arrivals reach into it
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+template <typename T, int BN>
+static cudaError_t launch_tile(const MatmulArgs& p, int split, int* status, cudaStream_t s)
+{
+    static SmemLimitSet set;
+    CUtensorMap w_map, a_map;
+    if (!token_byte_map(&w_map, p.w, p.K, p.N, p.w_stride, MM_K, 128, CU_TENSOR_MAP_SWIZZLE_128B)
+        || !token_byte_map(&a_map, p.a, p.K, p.M, p.a_stride, MM_K, BN, CU_TENSOR_MAP_SWIZZLE_128B))
+        return cudaErrorInvalidValue;
+    constexpr int STAGE = (128 + BN) * MM_K;
+    const int blocks = (p.K + MM_K - 1) / MM_K, room = TILE_RING / STAGE;
+    int stages = (blocks + split - 1) / split;
+    stages = stages < room ? stages : room;
+    stages = stages < 12 ? stages : 12;
+    const int part = split > 1 ? BN * 128 * 4 : 0;
+    const int bytes = (stages * STAGE > part ? stages * STAGE : part) + 1024;
+    const cudaError_t e = raise_smem_limit(matmul_i8_tile_kernel<T, BN>, set, TILE_RING + 1024);
+    if (e != cudaSuccess) return e;
+    const dim3 grid((unsigned)split, (unsigned)((p.N + 127) / 128), (unsigned)((p.M + BN - 1) / BN));
+    return launch_token(matmul_i8_tile_kernel<T, BN>, grid, 192, bytes, split, s, w_map, a_map, p, stages, status);
+}
+
+template <typename T>
+static cudaError_t launch_pair(const MatmulArgs& p, int sms, int* status, cudaStream_t s)
+{
+    static SmemLimitSet set;
+    CUtensorMap w_map, a_map;
+    if (!token_byte_map(&w_map, p.w, p.K, p.N, p.w_stride, MM_K, 128, CU_TENSOR_MAP_SWIZZLE_128B)
+        || !token_byte_map(&a_map, p.a, p.K, p.M, p.a_stride, MM_K, 128, CU_TENSOR_MAP_SWIZZLE_128B))
+        return cudaErrorInvalidValue;
+    const cudaError_t e = raise_smem_limit(matmul_i8_pair_kernel<T>, set, PAIR_SMEM);
+    if (e != cudaSuccess) return e;
+    const int tiles_n = (p.N + 255) / 256, tiles = tiles_n * ((p.M + 255) / 256);
+    const int pairs = tiles < sms / 2 ? tiles : sms / 2;
+    return launch_token(matmul_i8_pair_kernel<T>, dim3((unsigned)(2 * pairs)), PAIR_THREADS, PAIR_SMEM, 2, s, w_map, a_map, p, tiles_n, tiles, status);
+}
+
+// Cycles that a call is expected to take, by the number of tokens of a tile and of blocks that share one (0 tokens: pairs)
+static long long expected_cycles(const MatmulArgs& p, int sms, int bn, int split)
+{
+    const long long blocks = (p.K + MM_K - 1) / MM_K;
+    if (bn == 0) {
+        const long long tiles = (long long)((p.N + 255) / 256) * ((p.M + 255) / 256), waves = (tiles + sms / 2 - 1) / (sms / 2);
+        return waves * blocks * 512 + 6000;
+    }
+    const long long ctas = (long long)((p.N + 127) / 128) * ((p.M + bn - 1) / bn) * split, waves = (ctas + sms - 1) / sms;
+    // a step's MMAs (128 cycles for 256 tokens, no fewer than 50), or its bytes at 71 a cycle
+    const long long mma = bn >= 128 ? bn * 2 : 200, load = (128 + bn) * MM_K / 71;
+    return waves * ((blocks + split - 1) / split * (mma > load ? mma : load) + 3500 + bn * 8) + (split > 1 ? 1200 + bn * 12 : 0);
+}
+
 template <typename T>
 static cudaError_t launch_matmul(const MatmulArgs& p, cudaStream_t s)
 {
+    if (token_aligned(p.a, 16) && token_aligned(p.w, 16) && p.a_stride % 16 == 0 && p.w_stride % 16 == 0) {
+        int* const status = token_status_word();
+        if (!status) return cudaErrorInvalidSymbol;
+        const int sms = token_sms(), blocks = (p.K + MM_K - 1) / MM_K;
+        int best_bn = 0, best_split = 1;
+        long long best = p.M > 128 ? expected_cycles(p, sms, 0, 1) : 1ll << 62;
+        for (int bn = 16; bn <= 256; bn *= 2) {
+            if ((p.M + bn - 1) / bn > 65535) continue;
+            for (int split = 1; split <= 8 && split <= blocks; split *= 2) {
+                const long long c = expected_cycles(p, sms, bn, split);
+                if (c < best) { best = c; best_bn = bn; best_split = split; }
+            }
+            if (bn >= p.M) break;
+        }
+        switch (best_bn) {
+        case 0: return launch_pair<T>(p, sms, status, s);
+        case 16: return launch_tile<T, 16>(p, best_split, status, s);
+        case 32: return launch_tile<T, 32>(p, best_split, status, s);
+        case 64: return launch_tile<T, 64>(p, best_split, status, s);
+        case 128: return launch_tile<T, 128>(p, best_split, status, s);
+        default: return launch_tile<T, 256>(p, best_split, status, s);
+        }
+    }
     const dim3 grid((unsigned)((p.N + 63) / 64), (unsigned)((p.M + 63) / 64));
     return launch_token(matmul_i8_any_kernel<T>, grid, 256, 0, 1, s, p);
 }
