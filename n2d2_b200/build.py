@@ -12,7 +12,7 @@ SOURCES = ['net.cu', 'simt_kernels.cu', 'depthwise3x3.cu', 'igemm_tcgen05.cu', '
            'igemm_chain.cu', 'igemm_chain_float.cu', 'igemm_chain_any.cu', 'stem_tcgen05.cu', 'patch_tcgen05.cu', 'patch_float.cu', 'patch_wide.cu',
            'stem_s2d_tcgen05.cu', 'stem_s2d_pool.cu', 'stem_pool_tcgen05.cu', 'stem_pool_int.cu', 'stem_pool_float.cu',
            'stem_pool_wide.cu', 'small_net.cu', 'dwpw_tcgen05.cu', 'dwpw_forms.cu', 'probe_tcgen05.cu',
-           'token_norm.cu', 'token_matmul.cu', 'kv_append.cu', 'kv_attention.cu']
+           'token_norm.cu', 'token_matmul.cu', 'kv_append.cu', 'kv_attention.cu', 'kv_attention_prompt.cu']
 HEADERS = ['common.cuh', 'kernels.h', 'tc_common.cuh', 'host_internal.h', 'igemm_kernel.cuh', 'igemm_dual_kernel.cuh', 'igemm_chain_kernel.cuh',
            'patch_kernel.cuh', 'stem_pool_kernel.cuh', 'stem_s2d_kernel.cuh',
            'dwpw_kernel.cuh', 'token_common.cuh', 'kv_common.cuh', os.path.join('..', '..', 'include', 'n2d2b.h')]

@@ -18,34 +18,10 @@
 
 namespace n2d2b {
 
-struct AttendArgs {
-    KvArgs c;
-    const void* q;
-    void* out;
-    long long q_stride, out_stride;
-    float scale_log2;      // scale * log2(e)
-    int group;             // query heads of a key head
-    int causal, window;
-    int log_page;
-    int* status;
-};
-
 __device__ __forceinline__ void mma_f16(float* d, const unsigned* a, unsigned b0, unsigned b1)
 {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// (bytes 0, 1) and (bytes 2, 3) of four codes + 128 as halves 1024 + u
-__device__ __forceinline__ unsigned splice(unsigned w, unsigned sel)
-{
-    unsigned r;
-    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(w), "r"(0x64646464u), "r"(sel));
-    return r;
-}
-__device__ __forceinline__ unsigned less_1152(unsigned h)
-{
-    const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half(0x6480)));
-    return *reinterpret_cast<const unsigned*>(&d);
 }
 __device__ __forceinline__ uint4 lds128(unsigned addr)
 {
@@ -58,17 +34,6 @@ __device__ __forceinline__ uint2 lds64(unsigned addr)
     uint2 v;
     asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
     return v;
-}
-__device__ __forceinline__ float exp2_approx(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ unsigned pack_half2(float a, float b)
-{
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const unsigned*>(&h);
 }
 __device__ __forceinline__ float ld_cluster(unsigned addr)
 {
@@ -92,31 +57,6 @@ template <int D> struct RowsSmem {
     static constexpr int BYTES = RING + 1024;                          // the parts take the ring's place
     static_assert((ROWS_WARPS + 1) * PART + 4096 <= RING, "parts fit in the ring");
 };
-
-// One page's number and scales for a lane's unit half; what no query may see has no scale
-struct PageOf {
-    int number;
-    float k_scale, v_log, v_inverse;
-};
-__device__ __forceinline__ PageOf page_of(const KvArgs& c, int b, int head, int page, bool wanted)
-{
-    PageOf r = {0, 0.0f, 0.0f, 0.0f};
-    if (wanted) {
-        const float none = __int_as_float(0x7fffffff);
-        const int number = page < c.row ? c.table[(size_t)b * c.row + page] : -1;
-        if (number < 0 || number >= c.nb_pages) {
-            r.k_scale = none;
-        } else {
-            r.number = number;
-            r.k_scale = c.k_scales[(size_t)number * c.heads + head];
-            float v = c.v_scales[(size_t)number * c.heads + head];
-            if (v <= TOKEN_TINY) v = TOKEN_TINY;       // all codes are 0 then; any scale does
-            r.v_log = __log2f(v);
-            r.v_inverse = exp2_approx(-r.v_log);
-        }
-    }
-    return r;
-}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(ROWS_WARPS * 32, 2) kv_attention_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
@@ -317,7 +257,7 @@ __global__ void __launch_bounds__(ROWS_WARPS * 32, 2) kv_attention_rows_kernel(c
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float p = exp2_approx(sc[n][e] - base[e >> 1]);
-                sum[e >> 1] = fmaf(p, inv, sum[e >> 1]);
+                sum[e >> 1] = p == 0.0f ? sum[e >> 1] : fmaf(p, inv, sum[e >> 1]);   // (the scale of a page that a row does not see may be anything)
                 sc[n][e] = p;
             }
         }
@@ -457,9 +397,15 @@ static cudaError_t launch_rows(const CUtensorMap& k_map, const CUtensorMap& v_ma
                         k_map, v_map, a);
 }
 
+template <typename T> struct Half { static constexpr bool value = false; };
+template <> struct Half<__half> { static constexpr bool value = true; };
+
 template <typename T>
 static cudaError_t launch_attention(const n2d2b_kv_cache& cache, const AttendArgs& a, int sequences, cudaStream_t s)
 {
+    // from here on the tensor cores' tiles of 128 rows are filled well enough
+    if ((long long)a.c.max_new * a.group > 64 && sequences * (long long)a.c.heads * (((long long)a.c.max_new * a.group + 255) / 256) < (1ll << 31))
+        return launch_attention_prompt(a, cache.head_size, Half<T>::value, sequences, s);
     CUtensorMap k_map, v_map;
     const unsigned long long rows = (unsigned long long)cache.nb_pages * cache.nb_heads * cache.page_tokens;
     const unsigned box = cache.page_tokens < ROWS_UNIT ? 16 : ROWS_UNIT;

@@ -1,0 +1,409 @@
+// Attention of many new tokens over the paged 8-bit cache, on the tensor cores (the mathematics: kv_attention.cu).
+//
+// A block takes 256 rows (new token x query head of one key head, two tiles of 128) and walks over the tokens they see, 128 at a time.
+//   warps 4-7    bring pages through registers and write their codes as halves (exact) where the MMAs read them, swizzled
+//   warp 0       issues the MMAs: S = Q K^T (128 x 128, 32-bit sums in TMEM), O += P V with P read from TMEM in S's place
+//   warps 8-15   a thread holds one row of one tile: scores to probabilities, running maximum and sum, at the end O / sum
+// While the tensor pipe works on one tile, the other tile's rows are in the hands of their threads.  The output is only rescaled when a row's
+// maximum has grown by more than 2^8: below that the probabilities stay far inside 16 bits and their sum in 32 whatever the maximum they are
+// taken against.
+#include <cstdio>
+#include <cstring>
+#include "kv_common.cuh"
+
+namespace n2d2b {
+
+static constexpr int PR_THREADS = 512, PR_BLOCK = 128, PR_CONSTS = 4;
+template <int D> struct PromptSmem {
+    static constexpr int TILE = 128 * D * 2;                 // 128 rows (or tokens) of halves, in blocks of 64 columns
+    static constexpr int Q = 0, K = Q + 2 * TILE, V = K + 2 * TILE, BYTES = V + 2 * TILE + 1024;
+};
+
+__device__ __forceinline__ void tc_mma_f16_ss(unsigned d_tmem, unsigned a_lo, unsigned b_lo, unsigned desc_hi, unsigned idesc, unsigned accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "mov.b64 da, {%1, %3};\n\t"
+        "mov.b64 db, {%2, %3};\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tc_mma_f16_ts(unsigned d_tmem, unsigned a_tmem, unsigned b_lo, unsigned desc_hi, unsigned idesc, unsigned accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+        "mov.b64 db, {%2, %3};\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tc_st8(unsigned taddr, const unsigned* v)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
+__device__ __forceinline__ void tc_st32(unsigned taddr, const unsigned* v)
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+        ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+        "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]),
+        "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]) : "memory");
+}
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void sts128(unsigned addr, unsigned x, unsigned y, unsigned z, unsigned w)
+{
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+template <bool M> struct Masked { static constexpr bool value = M; };
+
+struct PromptBars {
+    unsigned long long k_full[2], k_empty[2], v_full[2], v_empty[2], q_full[2], s_full[2], p_full[2], o_full[2], c_full[PR_CONSTS];
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(PR_THREADS, 1) kv_attention_prompt_kernel(const AttendArgs a, int tiles, int sequences)
+{
+    typedef PromptSmem<D> S;
+    unsigned char* const smem = (unsigned char*)(((uintptr_t)dyn_smem() + 1023) & ~(uintptr_t)1023);
+    __shared__ __align__(8) PromptBars bars;
+    __shared__ float4 consts[PR_CONSTS][PR_BLOCK / 16];     // scale of the keys, log2 and reciprocal of the values', for 16 tokens
+    __shared__ unsigned tmem_slot;
+    __shared__ int abort_flag;
+    pdl_launch_dependents();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&bars.k_full[i]), 4);
+            mbar_init(smem_u32(&bars.v_full[i]), 4);
+            mbar_init(smem_u32(&bars.q_full[i]), 4);
+            mbar_init(smem_u32(&bars.p_full[i]), 4);
+            mbar_init(smem_u32(&bars.k_empty[i]), 1);
+            mbar_init(smem_u32(&bars.v_empty[i]), 1);
+            mbar_init(smem_u32(&bars.s_full[i]), 1);
+            mbar_init(smem_u32(&bars.o_full[i]), 1);
+        }
+        for (int i = 0; i < PR_CONSTS; ++i) mbar_init(smem_u32(&bars.c_full[i]), 1);
+        abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const unsigned tmem = tmem_slot;
+    pdl_wait();
+
+    // the rows with the most to see come first
+    const int head = (int)(blockIdx.x % (unsigned)a.c.heads), b = (int)(blockIdx.x / (unsigned)a.c.heads % (unsigned)sequences);
+    const int tile = tiles - 1 - (int)(blockIdx.x / (unsigned)a.c.heads / (unsigned)sequences);
+    const KvSequence s = kv_sequence(a.c, b);
+    const int row0 = tile * 256, rows = s.count * a.group - row0;
+    const bool any = rows > 0, two = rows > 128;
+    const int t_first = row0 / a.group, t_last = (min(row0 + 256, s.count * a.group) - 1) / a.group;
+    int lo = 0, hi = any ? s.length : 0;
+    if (a.causal) {
+        hi = min(hi, s.begin + t_last + 1);
+        if (a.window) lo = max(0, s.begin + t_first + 1 - a.window);
+    }
+    const int capacity = a.c.row << a.log_page;
+    hi = min(hi, capacity);
+    const int j_lo = lo / PR_BLOCK, blocks = hi > lo ? (hi + PR_BLOCK - 1) / PR_BLOCK - j_lo : 0;
+    const unsigned base = smem_u32(smem);
+
+    if (warp < 4) {
+        fewer_registers<40>();
+        if (warp == 0 && blocks > 0) {
+            const unsigned hi_k = (unsigned)(make_smem_desc(0u, 128) >> 32);
+            const unsigned idesc_s = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+            const unsigned idesc_o = (1u << 4) | (1u << 16) | (((unsigned)D >> 3) << 17) | ((128u >> 4) << 24);   // values: tokens are rows
+            const unsigned q_lo = ((base + S::Q) & 0x3ffffu) >> 4, k_lo = ((base + S::K) & 0x3ffffu) >> 4, v_lo = ((base + S::V) & 0x3ffffu) >> 4;
+            const int n = two ? 2 : 1;
+            auto scores = [&](int i, int j) {       // S of tile i, block j
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k) {
+                        const unsigned at = (unsigned)((k >> 2) * 1024 + (k & 3) * 2);
+                        tc_mma_f16_ss(tmem + (unsigned)(i * 128), q_lo + (unsigned)(i * (S::TILE / 16)) + at, k_lo + (unsigned)((j & 1) * (S::TILE / 16)) + at, hi_k,
+                                      idesc_s, k > 0);
+                    }
+                    tc_commit(smem_u32(&bars.s_full[i]));
+                    if (i == n - 1) tc_commit(smem_u32(&bars.k_empty[j & 1]));
+                }
+                __syncwarp();
+            };
+            bool ok = true;
+            for (int i = 0; i < n && ok; ++i) ok = mbar_wait_issuer(smem_u32(&bars.q_full[i]), 0, &abort_flag, a.status, 41);
+            if (ok) ok = mbar_wait_issuer(smem_u32(&bars.k_full[0]), 0, &abort_flag, a.status, 42);
+            if (ok) {
+                tc_fence_after();
+                for (int i = 0; i < n; ++i) scores(i, 0);
+            }
+            for (int j = 0; j < blocks && ok; ++j) {
+                ok = mbar_wait_issuer(smem_u32(&bars.v_full[j & 1]), (unsigned)(j >> 1) & 1u, &abort_flag, a.status, 43);
+                if (ok && j + 1 < blocks) ok = mbar_wait_issuer(smem_u32(&bars.k_full[(j + 1) & 1]), (unsigned)((j + 1) >> 1) & 1u, &abort_flag, a.status, 42);
+                for (int i = 0; i < n && ok; ++i) {
+                    ok = mbar_wait_issuer(smem_u32(&bars.p_full[i]), (unsigned)j & 1u, &abort_flag, a.status, 44);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < PR_BLOCK / 16; ++k)
+                            tc_mma_f16_ts(tmem + 256u + (unsigned)(i * 128), tmem + (unsigned)(i * 128 + k * 8),
+                                          (v_lo + (unsigned)((j & 1) * (S::TILE / 16)) + (unsigned)(k * 128)) | (1024u << 16), hi_k, idesc_o, j > 0 || k > 0);
+                        if (i == n - 1) tc_commit(smem_u32(&bars.v_empty[j & 1]));
+                        if (j == blocks - 1) tc_commit(smem_u32(&bars.o_full[i]));
+                    }
+                    __syncwarp();
+                    // (in order behind the product that reads P where this writes S)
+                    if (j + 1 < blocks) scores(i, j + 1);
+                }
+            }
+        }
+    } else if (warp < 8) {
+        fewer_registers<104>();
+        const int tid = threadIdx.x - 128;
+        constexpr int CHUNKS = D / 16, ROWS = 128 / CHUNKS, PASSES = 128 / ROWS;   // 16 codes a chunk, tokens of a pass, passes of a block
+        const int row = tid / CHUNKS, chunk = tid % CHUNKS;
+        PageOf held;        // lane i: tokens 16 i .. 16 i + 15 of the next block
+        auto fetch = [&](int j) {
+            const int token = (j_lo + j) * PR_BLOCK + lane * 16;
+            held = page_of(a.c, b, head, token >> a.log_page, lane < 8 && j < blocks && token < hi);
+        };
+        auto load = [&](uint4* r, const int8_t* from) {
+#pragma unroll
+            for (int i = 0; i < PASSES; ++i) {
+                const int t = i * ROWS + row;          // token of the block
+                const int number = __shfl_sync(0xffffffffu, held.number, t >> 4);
+                const int place = t & ((1 << a.log_page) - 1);
+                const size_t line = (((size_t)number * a.c.heads + head) << a.log_page) + (size_t)place;
+                r[i] = *reinterpret_cast<const uint4*>(from + line * D + chunk * 16);
+            }
+        };
+        // chunk of 16 halves pairs inside a row's 64-column block; lanes of the second block write in the other order: no two on one bank
+        const unsigned flip = (unsigned)(chunk >> 2) & 1u;
+        auto store = [&](const uint4* r, unsigned at) {
+#pragma unroll
+            for (int i = 0; i < PASSES; ++i) {
+                const int t = i * ROWS + row;
+                const unsigned w[4] = {r[i].x ^ 0x80808080u, r[i].y ^ 0x80808080u, r[i].z ^ 0x80808080u, r[i].w ^ 0x80808080u};
+                unsigned h[8];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { h[2 * e] = less_1152(splice(w[e], 0x4140)); h[2 * e + 1] = less_1152(splice(w[e], 0x4342)); }
+                const unsigned line = at + (unsigned)((chunk >> 2) * 16384 + t * 128);
+                const unsigned c0 = (((unsigned)(chunk & 3) * 2 + flip) ^ (unsigned)(t & 7)) << 4, c1 = (((unsigned)(chunk & 3) * 2 + 1 - flip) ^ (unsigned)(t & 7)) << 4;
+                sts128(line + c0, flip ? h[4] : h[0], flip ? h[5] : h[1], flip ? h[6] : h[2], flip ? h[7] : h[3]);
+                sts128(line + c1, flip ? h[0] : h[4], flip ? h[1] : h[5], flip ? h[2] : h[6], flip ? h[3] : h[7]);
+            }
+        };
+        uint4 k[PASSES], v[PASSES];
+        bool ok = true;
+        if (blocks > 0) {
+            fetch(0);
+            load(k, a.c.k);
+            load(v, a.c.v);
+        }
+        for (int j = 0; j < blocks && ok; ++j) {
+            // (the scores of block j - 2 came behind the probabilities of block j - 3: nobody reads the constants of block j - 4 any more)
+            if (j >= 2) ok = mbar_wait_warp(smem_u32(&bars.k_empty[j & 1]), (unsigned)((j >> 1) - 1) & 1u, &abort_flag, a.status, 45);
+            if (!ok) break;
+            if (warp == 4 && lane < 8) consts[j & (PR_CONSTS - 1)][lane] = make_float4(held.k_scale, held.v_log, held.v_inverse, 0.0f);
+            if (warp == 4) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&bars.c_full[j & (PR_CONSTS - 1)]));
+            }
+            store(k, base + S::K + (unsigned)((j & 1) * S::TILE));
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&bars.k_full[j & 1]));
+            fetch(j + 1);
+            if (j + 1 < blocks) load(k, a.c.k);
+            if (j >= 2) ok = mbar_wait_warp(smem_u32(&bars.v_empty[j & 1]), (unsigned)((j >> 1) - 1) & 1u, &abort_flag, a.status, 46);
+            if (!ok) break;
+            store(v, base + S::V + (unsigned)((j & 1) * S::TILE));
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&bars.v_full[j & 1]));
+            if (j + 1 < blocks) load(v, a.c.v);
+        }
+    } else {
+        more_registers<184>();
+        const int i = (warp - 8) >> 2, r = threadIdx.x - 256 - i * 128;      // tile and row
+        const int row = row0 + i * 128 + r, t = row / a.group, h = row - t * a.group;
+        const bool there = row < s.count * a.group;
+        const int pos = s.begin + t;
+        int see_lo = 0, see_hi = 0;
+        if (there) {
+            see_hi = a.causal ? min(s.length, pos + 1) : s.length;
+            if (a.causal && a.window) see_lo = max(0, pos + 1 - a.window);
+        }
+        float sum = there && see_hi > capacity ? __int_as_float(0x7fffffff) : 0.0f, top = -INFINITY, row_scale = 0.0f;
+        if (blocks > 0 && (i == 0 || two)) {
+            uint4 w[D / 8];
+            const T* const q = (const T*)a.q + (size_t)(s.first_row + t) * a.q_stride + (size_t)(head * a.group + h) * D;
+#pragma unroll
+            for (int e = 0; e < D / 8; ++e) {
+                w[e] = make_uint4(0, 0, 0, 0);
+                if (there) w[e] = *reinterpret_cast<const uint4*>(q + 8 * e);
+            }
+            unsigned largest = 0;
+#pragma unroll
+            for (int e = 0; e < D / 8; ++e) {
+                float f[8];
+                Elem<T>::unpack(w[e], f);
+#pragma unroll
+                for (int x = 0; x < 8; ++x) largest = max(largest, magnitude(f[x]));
+            }
+            // a power of two brings the row's largest value into [1, 4); the sign of the scale goes with it
+            const int exponent = min((int)(largest >> 23), 253);
+            const bool scaled = exponent > 0 && largest < 0x7f800000u;
+            const float up = copysignf(scaled ? __int_as_float((254 - exponent) << 23) : 1.0f, a.scale_log2);
+            row_scale = fabsf(a.scale_log2) * (scaled ? __int_as_float(exponent << 23) : 1.0f);
+#pragma unroll
+            for (int e = 0; e < D / 8; ++e) {
+                float f[8];
+                Elem<T>::unpack(w[e], f);
+                sts128(base + S::Q + (unsigned)(i * S::TILE + (e >> 3) * 16384 + r * 128 + (((e & 7) ^ (r & 7)) << 4)), pack_half2(f[0] * up, f[1] * up),
+                       pack_half2(f[2] * up, f[3] * up), pack_half2(f[4] * up, f[5] * up), pack_half2(f[6] * up, f[7] * up));
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&bars.q_full[i]));
+        }
+        const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
+        const unsigned s_at = tmem + lanes + (unsigned)(i * 128), o_at = tmem + lanes + 256u + (unsigned)(i * 128);
+        bool ok = true;
+        if (i == 0 || two) {
+            for (int j = 0; j < blocks; ++j) {
+                const int j0 = (j_lo + j) * PR_BLOCK;
+                ok = mbar_wait_warp(smem_u32(&bars.c_full[j & (PR_CONSTS - 1)]), (unsigned)(j / PR_CONSTS) & 1u, &abort_flag, a.status, 47)
+                     && mbar_wait_warp(smem_u32(&bars.s_full[i]), (unsigned)j & 1u, &abort_flag, a.status, 48);
+                if (!ok) break;
+                tc_fence_after();
+                unsigned x[128];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tc_ld32(s_at + 32u * c, x + 32 * c);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tc_wait_ld_into(x + 32 * c);
+                const float4* const group = consts[j & (PR_CONSTS - 1)];
+                // what a row does not see becomes -inf (only where a row of the warp sees less than the whole block)
+                const bool whole = see_lo <= j0 && see_hi >= j0 + PR_BLOCK;
+                const bool all_whole = __all_sync(0xffffffffu, whole);
+                if (!all_whole) {
+                    const unsigned first = (unsigned)(see_lo - j0), span = (unsigned)max(see_hi - see_lo, 0);
+#pragma unroll
+                    for (int c = 0; c < 128; ++c)
+                        if ((unsigned)c - first >= span) x[c] = 0xff800000u;
+                }
+                float best = top;
+#pragma unroll
+                for (int g = 0; g < 8; ++g) {
+                    float m = __uint_as_float(x[16 * g]);
+#pragma unroll
+                    for (int e = 1; e < 16; ++e) m = fmaxf(m, __uint_as_float(x[16 * g + e]));
+                    const float4 f = group[g];
+                    best = fmaxf(best, m == -INFINITY ? -INFINITY : fmaf(m, f.x * row_scale, f.y));
+                }
+                const bool grown = best > top + 8.0f || (top == -INFINITY && best > top);
+                if (__any_sync(0xffffffffu, grown)) {
+                    const float fade = grown ? exp2_approx(top - best) : 1.0f;
+                    if (grown) top = best;
+                    sum *= fade;
+                    if (j > 0) {
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 32) {
+                            unsigned o[32];
+                            tc_ld32(o_at + (unsigned)c, o);
+                            tc_wait_ld_into(o);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fade);
+                            tc_st32(o_at + (unsigned)c, o);
+                        }
+                    }
+                }
+                const float from = top == -INFINITY ? 0.0f : top;
+                auto probabilities = [&](auto masked) {
+#pragma unroll
+                    for (int g = 0; g < 8; ++g) {
+                        const float4 f = group[g];
+                        const float by = f.x * row_scale, add = f.y - from;
+                        float part = 0.0f;
+                        unsigned packed[8];
+#pragma unroll
+                        for (int e = 0; e < 16; e += 2) {
+                            float p[2];
+#pragma unroll
+                            for (int y = 0; y < 2; ++y) {
+                                const float v = __uint_as_float(x[16 * g + e + y]);
+                                p[y] = exp2_approx(fmaf(v, by, add));
+                                if (decltype(masked)::value) p[y] = v == -INFINITY ? 0.0f : p[y];   // (whatever the scales of a page it does not see)
+                            }
+                            part += p[0] + p[1];
+                            packed[e >> 1] = pack_half2(p[0], p[1]);
+                        }
+                        if (!decltype(masked)::value || part != 0.0f) sum = fmaf(part, f.z, sum);
+                        tc_st8(s_at + (unsigned)(8 * g), packed);
+                    }
+                };
+                if (all_whole) probabilities(Masked<false>());
+                else probabilities(Masked<true>());
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&bars.p_full[i]));
+            }
+            if (ok && blocks > 0) ok = mbar_wait_warp(smem_u32(&bars.o_full[i]), 0, &abort_flag, a.status, 49);
+            tc_fence_after();
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            T* const out = (T*)a.out + (size_t)(s.first_row + t) * a.out_stride + (size_t)(head * a.group + h) * D;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+                unsigned o[32];
+                tc_ld32(o_at + (unsigned)c, o);
+                tc_wait_ld_into(o);
+                if (there) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) {
+                        float f[8];
+#pragma unroll
+                        for (int y = 0; y < 8; ++y) f[y] = sum == 0.0f ? 0.0f : __uint_as_float(o[e + y]) * inv;
+                        *reinterpret_cast<uint4*>(out + c + e) = Elem<T>::pack(f);
+                    }
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+template <typename T, int D>
+static cudaError_t launch_prompt_of(const AttendArgs& a, int sequences, cudaStream_t s)
+{
+    static SmemLimitSet set;
+    const cudaError_t e = raise_smem_limit(kv_attention_prompt_kernel<T, D>, set, PromptSmem<D>::BYTES);
+    if (e != cudaSuccess) return e;
+    const long long tiles = ((long long)a.c.max_new * a.group + 255) / 256;
+    return launch_token(kv_attention_prompt_kernel<T, D>, dim3((unsigned)(tiles * a.c.heads * sequences)), PR_THREADS, PromptSmem<D>::BYTES, 1, s, a, (int)tiles, sequences);
+}
+
+cudaError_t launch_attention_prompt(const AttendArgs& a, int head_size, bool half, int sequences, cudaStream_t s)
+{
+    if (half) return head_size == 64 ? launch_prompt_of<__half, 64>(a, sequences, s) : launch_prompt_of<__half, 128>(a, sequences, s);
+    return head_size == 64 ? launch_prompt_of<__nv_bfloat16, 64>(a, sequences, s) : launch_prompt_of<__nv_bfloat16, 128>(a, sequences, s);
+}
+
+}  // namespace n2d2b

@@ -63,4 +63,68 @@ static inline int kv_check(const n2d2b_kv_cache* cache, const n2d2b_kv_batch* ba
     return 0;
 }
 
+// ----------------------------------------------------------------------------- attention
+struct AttendArgs {
+    KvArgs c;
+    const void* q;
+    void* out;
+    long long q_stride, out_stride;
+    float scale_log2;      // scale * log2(e)
+    int group;             // query heads of a key head
+    int causal, window;
+    int log_page;
+    int* status;
+};
+
+// (bytes 0, 1) and (bytes 2, 3) of four codes + 128 as halves 1024 + u
+__device__ __forceinline__ unsigned splice(unsigned w, unsigned sel)
+{
+    unsigned r;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(w), "r"(0x64646464u), "r"(sel));
+    return r;
+}
+__device__ __forceinline__ unsigned less_1152(unsigned h)
+{
+    const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half(0x6480)));
+    return *reinterpret_cast<const unsigned*>(&d);
+}
+__device__ __forceinline__ float exp2_approx(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ unsigned pack_half2(float a, float b)
+{
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const unsigned*>(&h);
+}
+// One page's number and scales for a lane's unit half; what no query may see has no scale
+struct PageOf {
+    int number;
+    float k_scale, v_log, v_inverse;
+};
+__device__ __forceinline__ PageOf page_of(const KvArgs& c, int b, int head, int page, bool wanted)
+{
+    PageOf r = {0, 0.0f, 0.0f, 0.0f};
+    if (wanted) {
+        const float none = __int_as_float(0x7fffffff);
+        const int number = page < c.row ? c.table[(size_t)b * c.row + page] : -1;
+        if (number < 0 || number >= c.nb_pages) {
+            r.k_scale = none;
+        } else {
+            r.number = number;
+            r.k_scale = c.k_scales[(size_t)number * c.heads + head];
+            float v = c.v_scales[(size_t)number * c.heads + head];
+            if (v <= TOKEN_TINY) v = TOKEN_TINY;       // all codes are 0 then; any scale does
+            r.v_log = __log2f(v);
+            r.v_inverse = exp2_approx(-r.v_log);
+        }
+    }
+    return r;
+}
+
+// Many rows of a key head on the tensor cores (kv_attention_prompt.cu)
+cudaError_t launch_attention_prompt(const AttendArgs& a, int head_size, bool half, int sequences, cudaStream_t s);
+
 }  // namespace n2d2b

@@ -439,6 +439,20 @@ def test_attention_what_is_no_number_stays_in_its_row(new):
     assert torch.equal(out[same], clean[same])
 
 
+@pytest.mark.parametrize('which', ['k_scales', 'v_scales'])
+@pytest.mark.parametrize('page, new, heads', [(16, 40, 1), (16, 12, 1), (64, 100, 2), (32, 60, 8), (128, 200, 4)])
+def test_attention_a_poisoned_page_reaches_those_who_see_it(page, new, heads, which):
+    s = Served([300], [new], 1, 128, page, 'bf16', heads=heads)
+    clean = s.attention()
+    last = 299 // page              # the page of the last token
+    getattr(s, which)[s.table[0][last]] = math.nan
+    out = s.attention()
+    unaware = max(0, min(new, last * page - (300 - new)))
+    assert torch.equal(out[:unaware], clean[:unaware])
+    assert out[unaware:new].isnan().all()
+    assert (out[new:] == 3).all()
+
+
 @pytest.mark.parametrize('bad', [-1, -2 ** 31, 2 ** 31 - 1, None])
 @pytest.mark.parametrize('news', [[1, 1, 1], [40, 5, 7]])
 @pytest.mark.parametrize('page', [16, 64])
