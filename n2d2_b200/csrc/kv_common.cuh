@@ -88,6 +88,9 @@ __device__ __forceinline__ unsigned less_1152(unsigned h)
     const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half(0x6480)));
     return *reinterpret_cast<const unsigned*>(&d);
 }
+// Codes in bytes 0 and 2 (1 and 3) of a word as two halves
+__device__ __forceinline__ unsigned widen_even(unsigned w) { return less_1152((w & 0x00ff00ffu) ^ 0x64806480u); }
+__device__ __forceinline__ unsigned widen_odd(unsigned w) { return less_1152(((w >> 8) & 0x00ff00ffu) ^ 0x64806480u); }
 __device__ __forceinline__ float exp2_approx(float x)
 {
     float y;
