@@ -383,8 +383,9 @@ int n2d2b_rmsnorm_quantize(int device, const n2d2b_norm* norm, n2d2b_stream stre
 
 /* Matrix product of 8-bit codes with a scale for each token (row of a) and each output channel (row of w):
  *   out[i][j] = (sum over k of a[i][k] * w[j][k]) * a_scales[i] * w_scales[j] + bias[j]
- * The sum is exact in 32 bits (k up to 131071; codes may be -128 here); the products with the scales and the bias are taken in 32
- * bits and rounded once to dtype.  Rows of a or w that do not start on 16 bytes (address or stride) take a slower kernel. */
+ * The sum is exact in 32 bits (k up to 131071; codes may be -128 here; m up to 4194240, n up to 8388480); the products with the scales and the bias are taken in 32
+ * bits and rounded once to dtype.  Rows of a or w that do not start on 16 bytes (address or stride) take a slower
+ * kernel, which reads whole words of four bytes: up to three bytes beside a row's ends, never stored nor counted. */
 typedef struct n2d2b_matmul {
     int32_t dtype;             /* of out: N2D2B_F32, N2D2B_F16 or N2D2B_BF16 */
     int32_t m, n, k;           /* tokens, output channels, input channels */

@@ -35,19 +35,6 @@ __device__ __forceinline__ uint2 lds64(unsigned addr)
     asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
     return v;
 }
-__device__ __forceinline__ float ld_cluster(unsigned addr)
-{
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-    return v;
-}
-__device__ __forceinline__ float4 ld_cluster4(unsigned addr)
-{
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-    return v;
-}
-
 static constexpr int ROWS_UNIT = 32;
 template <int D, int NT, int WARPS> struct RowsSmem {
     static constexpr int STAGES = 256 / D;
@@ -458,7 +445,7 @@ template <typename T>
 static cudaError_t launch_attention(const n2d2b_kv_cache& cache, const AttendArgs& a, int sequences, cudaStream_t s)
 {
     // from here on the tensor cores' tiles of 128 rows are filled well enough
-    if ((long long)a.c.max_new * a.group > 64 && sequences * (long long)a.c.heads * (((long long)a.c.max_new * a.group + 255) / 256) < (1ll << 31))
+    if ((long long)a.c.max_new * a.group > 64 && sequences * (long long)a.c.heads * (((long long)a.c.max_new * a.group + 255) / 256) < (1ll << 27))
         return launch_attention_prompt(a, cache.head_size, Half<T>::value, sequences, s);
     CUtensorMap k_map, v_map;
     const unsigned long long rows = (unsigned long long)cache.nb_pages * cache.nb_heads * cache.page_tokens;

@@ -17,6 +17,8 @@ static constexpr int PR_THREADS = 512, PR_BLOCK = 128, PR_CONSTS = 4;
 template <int D> struct PromptSmem {
     static constexpr int TILE = 128 * D * 2;                 // 128 rows (or tokens) of halves, in blocks of 64 columns
     static constexpr int Q = 0, K = Q + 2 * TILE, V = K + 2 * TILE, BYTES = V + 2 * TILE + 1024;
+    static constexpr int PITCH = D + 4;                      // floats of a row of a part, in the tiles' place at the end
+    static_assert(256 * PITCH * 4 <= 6 * TILE, "a part fits");
 };
 
 __device__ __forceinline__ void tc_mma_f16_ss(unsigned d_tmem, unsigned a_lo, unsigned b_lo, unsigned desc_hi, unsigned idesc, unsigned accumulate)
@@ -74,6 +76,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_attention_prompt_kernel(cons
     unsigned char* const smem = (unsigned char*)(((uintptr_t)dyn_smem() + 1023) & ~(uintptr_t)1023);
     __shared__ __align__(8) PromptBars bars;
     __shared__ float4 consts[PR_CONSTS][PR_BLOCK / 16];     // scale of the keys, log2 and reciprocal of the values', for 16 tokens
+    __shared__ float part_top[256], part_sum[256];
     __shared__ unsigned tmem_slot;
     __shared__ int abort_flag;
     pdl_launch_dependents();
@@ -104,8 +107,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_attention_prompt_kernel(cons
     pdl_wait();
 
     // the rows with the most to see come first
-    const int head = (int)(blockIdx.x % (unsigned)a.c.heads), b = (int)(blockIdx.x / (unsigned)a.c.heads % (unsigned)sequences);
-    const int tile = tiles - 1 - (int)(blockIdx.x / (unsigned)a.c.heads / (unsigned)sequences);
+    const unsigned rank = cluster_rank(), ranks = cluster_size(), id = blockIdx.x / ranks;
+    const int head = (int)(id % (unsigned)a.c.heads), b = (int)(id / (unsigned)a.c.heads % (unsigned)sequences);
+    const int tile = tiles - 1 - (int)(id / (unsigned)a.c.heads / (unsigned)sequences);
     const KvSequence s = kv_sequence(a.c, b);
     const int row0 = tile * 256, rows = s.count * a.group - row0;
     const bool any = rows > 0, two = rows > 128;
@@ -117,7 +121,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_attention_prompt_kernel(cons
     }
     const int capacity = a.c.row << a.log_page;
     hi = min(hi, capacity);
-    const int j_lo = lo / PR_BLOCK, blocks = hi > lo ? (hi + PR_BLOCK - 1) / PR_BLOCK - j_lo : 0;
+    // the blocks of a cluster take a part of the tokens each
+    const int all = hi > lo ? (hi + PR_BLOCK - 1) / PR_BLOCK - lo / PR_BLOCK : 0, per = (all + (int)ranks - 1) / (int)ranks;
+    const int j_lo = lo / PR_BLOCK + (int)rank * per, blocks = max(0, min(per, all - (int)rank * per));
     const unsigned base = smem_u32(smem);
 
     if (warp < 4) {
@@ -362,6 +368,23 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_attention_prompt_kernel(cons
                 if (lane == 0) mbar_arrive(smem_u32(&bars.p_full[i]));
             }
             if (ok && blocks > 0) ok = mbar_wait_warp(smem_u32(&bars.o_full[i]), 0, &abort_flag, a.status, 49);
+            if (ranks > 1) {
+                // the part goes where the tiles were: both tiles' products are through
+                if (ok && blocks > 0 && two) ok = mbar_wait_warp(smem_u32(&bars.o_full[i ^ 1]), 0, &abort_flag, a.status, 49);
+                tc_fence_after();
+                float* const to = (float*)smem + (size_t)(i * 128 + r) * S::PITCH;
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    unsigned o[32];
+                    tc_ld32(o_at + (unsigned)c, o);
+                    tc_wait_ld_into(o);
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4)
+                        *reinterpret_cast<uint4*>(to + c + e) = blocks > 0 ? make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]) : make_uint4(0, 0, 0, 0);
+                }
+                part_top[i * 128 + r] = top;
+                part_sum[i * 128 + r] = sum;
+            } else {
             tc_fence_after();
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             T* const out = (T*)a.out + (size_t)(s.first_row + t) * a.out_stride + (size_t)(head * a.group + h) * D;
@@ -380,10 +403,36 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_attention_prompt_kernel(cons
                     }
                 }
             }
+            }
         }
     }
     tc_fence_before();
     __syncthreads();
+    if (ranks > 1) {
+        cluster_sync();
+        // every block finishes a share of the outputs
+        const int there = max(0, min(rows, 256)) * (D / 4);
+        for (int e = (int)(rank * PR_THREADS + threadIdx.x); e < there; e += (int)ranks * PR_THREADS) {
+            const int r = e / (D / 4), d = e % (D / 4) * 4;
+            const unsigned at = base + (unsigned)(r * S::PITCH + d) * 4u, at_top = smem_u32(part_top + r), at_sum = smem_u32(part_sum + r);
+            float m = -INFINITY;
+            for (unsigned k = 0; k < ranks; ++k) m = fmaxf(m, ld_cluster(map_to_rank(at_top, k)));
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float l = 0.0f;
+            for (unsigned k = 0; k < ranks; ++k) {
+                const float t = ld_cluster(map_to_rank(at_top, k));
+                const float f = t == m ? 1.0f : exp2_approx(t - m);
+                const float4 x = ld_cluster4(map_to_rank(at, k));
+                o.x = fmaf(x.x, f, o.x); o.y = fmaf(x.y, f, o.y); o.z = fmaf(x.z, f, o.z); o.w = fmaf(x.w, f, o.w);
+                l = fmaf(ld_cluster(map_to_rank(at_sum, k)), f, l);
+            }
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            const int row = row0 + r, t = row / a.group, h = row - t * a.group;
+            T* const out = (T*)a.out + (size_t)(s.first_row + t) * a.out_stride + (size_t)(head * a.group + h) * D + d;
+            *reinterpret_cast<uint2*>(out) = make_uint2(Elem<T>::pack2(o.x * inv, o.y * inv), Elem<T>::pack2(o.z * inv, o.w * inv));
+        }
+        cluster_sync();     // no block leaves while another reads its part
+    }
     if (warp == 0) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
@@ -396,8 +445,12 @@ static cudaError_t launch_prompt_of(const AttendArgs& a, int sequences, cudaStre
     static SmemLimitSet set;
     const cudaError_t e = raise_smem_limit(kv_attention_prompt_kernel<T, D>, set, PromptSmem<D>::BYTES);
     if (e != cudaSuccess) return e;
-    const long long tiles = ((long long)a.c.max_new * a.group + 255) / 256;
-    return launch_token(kv_attention_prompt_kernel<T, D>, dim3((unsigned)(tiles * a.c.heads * sequences)), PR_THREADS, PromptSmem<D>::BYTES, 1, s, a, (int)tiles, sequences);
+    const long long tiles = ((long long)a.c.max_new * a.group + 255) / 256, blocks = tiles * a.c.heads * sequences;
+    const long long most = a.window ? min((long long)a.c.row << a.log_page, (long long)a.window + a.c.max_new) : (long long)a.c.row << a.log_page;
+    // where half of the multiprocessors would have nothing to do, clusters share the tokens, at least two steps to a block
+    int split = 1;
+    while (split < 8 && blocks * split * 2 <= token_sms() && split * 4 * PR_BLOCK <= most) split *= 2;
+    return launch_token(kv_attention_prompt_kernel<T, D>, dim3((unsigned)(blocks * split)), PR_THREADS, PromptSmem<D>::BYTES, split, s, a, (int)tiles, sequences);
 }
 
 cudaError_t launch_attention_prompt(const AttendArgs& a, int head_size, bool half, int sequences, cudaStream_t s)

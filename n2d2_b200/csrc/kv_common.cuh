@@ -102,6 +102,18 @@ __device__ __forceinline__ unsigned pack_half2(float a, float b)
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const unsigned*>(&h);
 }
+__device__ __forceinline__ float ld_cluster(unsigned addr)
+{
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 ld_cluster4(unsigned addr)
+{
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
 // One page's number and scales for a lane's unit half; what no query may see has no scale
 struct PageOf {
     int number;

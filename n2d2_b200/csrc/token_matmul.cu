@@ -17,59 +17,6 @@ struct MatmulArgs {
     int M, N, K;
 };
 
-template <typename T>
-__device__ __forceinline__ void store_scaled(const MatmulArgs& p, int i, int j, int acc, float sa, float sw, float bias)
-{
-    float v = (float)acc * sa * sw;
-    if (p.bias) v += bias;
-    ((T*)p.out)[(size_t)i * p.out_stride + j] = Elem<T>::from_float(v);
-}
-
-// Rows of any address and stride: 64 x 64 outputs a block, 4 x 4 a thread, 64 bytes of k a step through shared memory.
-template <typename T>
-__global__ void __launch_bounds__(256) matmul_i8_any_kernel(const MatmulArgs p)
-{
-    pdl_launch_dependents();
-    pdl_wait();
-    constexpr int PITCH = 17;   // words of a row: 16 and one against bank conflicts
-    __shared__ int as[64 * PITCH], ws[64 * PITCH];
-    const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    int acc[4][4] = {};
-    for (int k0 = 0; k0 < p.K; k0 += 64) {
-        for (int i = threadIdx.x; i < 2 * 64 * 64; i += 256) {
-            const int which = i >> 12, row = (i >> 6) & 63, k = k0 + (i & 63);
-            const int g = which ? n0 + row : m0 + row;
-            int8_t v = 0;
-            if (k < p.K && g < (which ? p.N : p.M)) v = which ? p.w[(size_t)g * p.w_stride + k] : p.a[(size_t)g * p.a_stride + k];
-            ((int8_t*)((which ? ws : as) + row * PITCH))[i & 63] = v;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-            int av[4], wv[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) { av[e] = as[(ty + 16 * e) * PITCH + k]; wv[e] = ws[(tx + 16 * e) * PITCH + k]; }
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int f = 0; f < 4; ++f) acc[e][f] = __dp4a(av[e], wv[f], acc[e][f]);
-        }
-        __syncthreads();
-    }
-#pragma unroll
-    for (int f = 0; f < 4; ++f) {
-        const int j = n0 + tx + 16 * f;
-        if (j >= p.N) continue;
-        const float sw = p.w_scales[j], bias = p.bias ? p.bias[j] : 0.0f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int i = m0 + ty + 16 * e;
-            if (i < p.M) store_scaled<T>(p, i, j, acc[e][f], p.a_scales[i], sw, bias);
-        }
-    }
-}
-
 // ----------------------------------------------------------------------------- tensor cores
 // Weights are the M operand of the MMAs (128 output channels to 128 TMEM lanes), tokens the N operand: a thread of the epilogue owns one output
 // channel (its scale and bias sit in registers), a warp stores 32 neighbouring channels of a token at a time, and a call of
@@ -90,9 +37,27 @@ __device__ __forceinline__ void store_columns(const MatmulArgs& p, const unsigne
     }
 }
 
+// 16 bytes of k of a row that starts anywhere, zero from byte `valid` on: aligned words that hold a wanted byte, shifted into place
+__device__ __forceinline__ uint4 load_bytes(const int8_t* p, int valid)
+{
+    const unsigned shift = (unsigned)((uintptr_t)p & 3u);
+    const unsigned* const w = reinterpret_cast<const unsigned*>((uintptr_t)p - shift);
+    unsigned x[5], r[4];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) x[i] = 4 * i < (int)shift + valid ? w[i] : 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        r[i] = __funnelshift_r(x[i], x[i + 1], 8u * shift);
+        const int left = valid - 4 * i;
+        r[i] = left >= 4 ? r[i] : (left <= 0 ? 0u : r[i] & (0xffffffffu >> (32 - 8 * left)));
+    }
+    return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
 // One tile of 128 channels x BN tokens a block.  Few tiles: the blocks of a cluster take parts of k and add their 32-bit sums up through
-// distributed shared memory, each finishing a share of the tile.  Warp 0 loads, warp 1 issues the MMAs, four warps store.
-template <typename T, int BN>
+// distributed shared memory, each finishing a share of the tile.  Warp 0 loads, warp 1 issues the MMAs, four warps store.  BYTES: rows that TMA cannot read (not on 16
+// bytes); the storing warps bring them through registers first.
+template <typename T, int BN, bool BYTES>
 __global__ void __launch_bounds__(192, 1) matmul_i8_tile_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap a_map, const MatmulArgs p,
                                                                 int stages, int* status)
 {
@@ -105,9 +70,8 @@ __global__ void __launch_bounds__(192, 1) matmul_i8_tile_kernel(const __grid_con
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        prefetch_tensor_map(&w_map);
-        prefetch_tensor_map(&a_map);
-        for (int i = 0; i < stages; ++i) { mbar_init(smem_u32(&full[i]), 1); mbar_init(smem_u32(&empty[i]), 1); }
+        if (!BYTES) { prefetch_tensor_map(&w_map); prefetch_tensor_map(&a_map); }
+        for (int i = 0; i < stages; ++i) { mbar_init(smem_u32(&full[i]), BYTES ? 4 : 1); mbar_init(smem_u32(&empty[i]), 1); }
         mbar_init(smem_u32(&done), 1);
         abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -127,7 +91,7 @@ __global__ void __launch_bounds__(192, 1) matmul_i8_tile_kernel(const __grid_con
     const int blocks = (p.K + MM_K - 1) / MM_K, per = (blocks + (int)ranks - 1) / (int)ranks;
     const int from = (int)rank * per, count = max(0, min(per, blocks - from));
     if (warp == 0) {
-        for (int i = 0; i < count; ++i) {
+        for (int i = 0; !BYTES && i < count; ++i) {
             const int slot = i % stages;
             if (i >= stages && !mbar_wait_issuer(smem_u32(&empty[slot]), (unsigned)(i / stages - 1) & 1u, &abort_flag, status, 31)) break;
             if (elect_one()) {
@@ -158,6 +122,34 @@ __global__ void __launch_bounds__(192, 1) matmul_i8_tile_kernel(const __grid_con
         }
     } else {
         for (int i = (int)threadIdx.x - 64; i < BN; i += 128) sa[i] = t0 + i < p.M ? p.a_scales[t0 + i] : 0.0f;
+        const int tid = (int)threadIdx.x - 64, chunk = tid & 7;
+        for (int i = 0; BYTES && i < count; ++i) {
+            const int slot = i % stages, k = (from + i) * MM_K + chunk * 16, valid = min(max(p.K - k, 0), 16);
+            if (i >= stages && !mbar_wait_warp(smem_u32(&empty[slot]), (unsigned)(i / stages - 1) & 1u, &abort_flag, status, 31)) break;
+            const unsigned dst = smem_u32(smem) + (unsigned)(slot * STAGE);
+            // rows tid / 8, + 16, ...: four at a time, so that their loads are under way together
+#pragma unroll 1
+            for (int r0 = tid >> 3; r0 < 128 + BN; r0 += 64) {
+                uint4 v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = r0 + 16 * e, row = r < 128 ? n0 + r : t0 + r - 128;
+                    const bool there = r < 128 + BN && row < (r < 128 ? p.N : p.M);
+                    const int8_t* const at = r < 128 ? p.w + (size_t)row * p.w_stride + k : p.a + (size_t)row * p.a_stride + k;
+                    v[e] = load_bytes(at, there ? valid : 0);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = r0 + 16 * e;
+                    if (r < 128 + BN)
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst + (unsigned)(r * MM_K + ((chunk ^ (r & 7)) << 4))), "r"(v[e].x), "r"(v[e].y),
+                                     "r"(v[e].z), "r"(v[e].w) : "memory");
+                }
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&full[slot]));
+        }
     }
     __syncthreads();
     const bool ok = count == 0 || mbar_wait_warp(smem_u32(&done), 0, &abort_flag, status, 33);
@@ -353,12 +345,13 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) matmul_i8_pair_kernel(const _
     }
 }
 
-template <typename T, int BN>
+template <typename T, int BN, bool BYTES>
 static cudaError_t launch_tile(const MatmulArgs& p, int split, int* status, cudaStream_t s)
 {
     static SmemLimitSet set;
-    CUtensorMap w_map, a_map;
-    if (!token_byte_map(&w_map, p.w, p.K, p.N, p.w_stride, MM_K, 128, CU_TENSOR_MAP_SWIZZLE_128B)
+    CUtensorMap w_map = {}, a_map = {};
+    if (BYTES) {
+    } else if (!token_byte_map(&w_map, p.w, p.K, p.N, p.w_stride, MM_K, 128, CU_TENSOR_MAP_SWIZZLE_128B)
         || !token_byte_map(&a_map, p.a, p.K, p.M, p.a_stride, MM_K, BN, CU_TENSOR_MAP_SWIZZLE_128B))
         return cudaErrorInvalidValue;
     constexpr int STAGE = (128 + BN) * MM_K;
@@ -368,10 +361,10 @@ static cudaError_t launch_tile(const MatmulArgs& p, int split, int* status, cuda
     stages = stages < 12 ? stages : 12;
     const int part = split > 1 ? BN * 128 * 4 : 0;
     const int bytes = (stages * STAGE > part ? stages * STAGE : part) + 1024;
-    const cudaError_t e = raise_smem_limit(matmul_i8_tile_kernel<T, BN>, set, TILE_RING + 1024);
+    const cudaError_t e = raise_smem_limit(matmul_i8_tile_kernel<T, BN, BYTES>, set, TILE_RING + 1024);
     if (e != cudaSuccess) return e;
     const dim3 grid((unsigned)split, (unsigned)((p.N + 127) / 128), (unsigned)((p.M + BN - 1) / BN));
-    return launch_token(matmul_i8_tile_kernel<T, BN>, grid, 192, bytes, split, s, w_map, a_map, p, stages, status);
+    return launch_token(matmul_i8_tile_kernel<T, BN, BYTES>, grid, 192, bytes, split, s, w_map, a_map, p, stages, status);
 }
 
 template <typename T>
@@ -390,7 +383,7 @@ static cudaError_t launch_pair(const MatmulArgs& p, int sms, int* status, cudaSt
 }
 
 // Cycles that a call is expected to take, by the number of tokens of a tile and of blocks that share one (0 tokens: pairs)
-static long long expected_cycles(const MatmulArgs& p, int sms, int bn, int split)
+static long long expected_cycles(const MatmulArgs& p, int sms, int bn, int split, bool bytes)
 {
     const long long blocks = (p.K + MM_K - 1) / MM_K;
     if (bn == 0) {
@@ -398,39 +391,42 @@ static long long expected_cycles(const MatmulArgs& p, int sms, int bn, int split
         return waves * blocks * 512 + 6000;
     }
     const long long ctas = (long long)((p.N + 127) / 128) * ((p.M + bn - 1) / bn) * split, waves = (ctas + sms - 1) / sms;
-    // a step's MMAs (128 cycles for 256 tokens, no fewer than 50), or its bytes at 71 a cycle
-    const long long mma = bn >= 128 ? bn * 2 : 200, load = (128 + bn) * MM_K / 71;
+    // a step's MMAs (128 cycles for 256 tokens, no fewer than 50), or its bytes at 71 a cycle (through registers: 16)
+    const long long mma = bn >= 128 ? bn * 2 : 200, load = (128 + bn) * MM_K / (bytes ? 16 : 71);
     return waves * ((blocks + split - 1) / split * (mma > load ? mma : load) + 3500 + bn * 8) + (split > 1 ? 1200 + bn * 12 : 0);
+}
+
+template <typename T, bool BYTES>
+static cudaError_t launch_tiles(const MatmulArgs& p, int bn, int split, int* status, cudaStream_t s)
+{
+    switch (bn) {
+    case 16: return launch_tile<T, 16, BYTES>(p, split, status, s);
+    case 32: return launch_tile<T, 32, BYTES>(p, split, status, s);
+    case 64: return launch_tile<T, 64, BYTES>(p, split, status, s);
+    case 128: return launch_tile<T, 128, BYTES>(p, split, status, s);
+    default: return launch_tile<T, 256, BYTES>(p, split, status, s);
+    }
 }
 
 template <typename T>
 static cudaError_t launch_matmul(const MatmulArgs& p, cudaStream_t s)
 {
-    if (token_aligned(p.a, 16) && token_aligned(p.w, 16) && p.a_stride % 16 == 0 && p.w_stride % 16 == 0) {
-        int* const status = token_status_word();
-        if (!status) return cudaErrorInvalidSymbol;
-        const int sms = token_sms(), blocks = (p.K + MM_K - 1) / MM_K;
-        int best_bn = 0, best_split = 1;
-        long long best = p.M > 128 ? expected_cycles(p, sms, 0, 1) : 1ll << 62;
-        for (int bn = 16; bn <= 256; bn *= 2) {
-            if ((p.M + bn - 1) / bn > 65535) continue;
-            for (int split = 1; split <= 8 && split <= blocks; split *= 2) {
-                const long long c = expected_cycles(p, sms, bn, split);
-                if (c < best) { best = c; best_bn = bn; best_split = split; }
-            }
-            if (bn >= p.M) break;
+    const bool bytes = !token_aligned(p.a, 16) || !token_aligned(p.w, 16) || p.a_stride % 16 || p.w_stride % 16;
+    int* const status = token_status_word();
+    if (!status) return cudaErrorInvalidSymbol;
+    const int sms = token_sms(), blocks = (p.K + MM_K - 1) / MM_K;
+    int best_bn = 0, best_split = 1;
+    long long best = p.M > 128 && !bytes ? expected_cycles(p, sms, 0, 1, false) : 1ll << 62;
+    for (int bn = 16; bn <= 256; bn *= 2) {
+        if ((p.M + bn - 1) / bn > 65535) continue;
+        for (int split = 1; split <= 8 && split <= blocks; split *= 2) {
+            const long long c = expected_cycles(p, sms, bn, split, bytes);
+            if (c < best) { best = c; best_bn = bn; best_split = split; }
         }
-        switch (best_bn) {
-        case 0: return launch_pair<T>(p, sms, status, s);
-        case 16: return launch_tile<T, 16>(p, best_split, status, s);
-        case 32: return launch_tile<T, 32>(p, best_split, status, s);
-        case 64: return launch_tile<T, 64>(p, best_split, status, s);
-        case 128: return launch_tile<T, 128>(p, best_split, status, s);
-        default: return launch_tile<T, 256>(p, best_split, status, s);
-        }
+        if (bn >= p.M) break;
     }
-    const dim3 grid((unsigned)((p.N + 63) / 64), (unsigned)((p.M + 63) / 64));
-    return launch_token(matmul_i8_any_kernel<T>, grid, 256, 0, 1, s, p);
+    if (best_bn == 0) return launch_pair<T>(p, sms, status, s);
+    return bytes ? launch_tiles<T, true>(p, best_bn, best_split, status, s) : launch_tiles<T, false>(p, best_bn, best_split, status, s);
 }
 
 }  // namespace n2d2b
@@ -445,6 +441,7 @@ extern "C" int n2d2b_matmul_i8(int device, const n2d2b_matmul* matmul, n2d2b_str
     if (d.m < 0 || d.n < 1 || d.k < 1) return set_error(N2D2B_ERR_INVALID, "invalid size: %d x %d x %d", d.m, d.n, d.k);
     if (d.k > 131071) return set_error(N2D2B_ERR_TOO_LARGE, "k = %d exceeds 131071, beyond which sums could leave 32 bits", d.k);
     if (d.m > 65535 * 64) return set_error(N2D2B_ERR_TOO_LARGE, "m = %d exceeds %d", d.m, 65535 * 64);
+    if (d.n > 65535 * 128) return set_error(N2D2B_ERR_TOO_LARGE, "n = %d exceeds %d", d.n, 65535 * 128);
     if (d.m == 0) return 0;
     if (!d.a || !d.a_scales || !d.w || !d.w_scales || !d.out) return set_error(N2D2B_ERR_INVALID, "a, w, their scales and out must not be NULL");
     if (!token_aligned(d.out, token_item(d.dtype)) || !token_aligned(d.a_scales, 4) || !token_aligned(d.w_scales, 4) || !token_aligned(d.bias, 4))

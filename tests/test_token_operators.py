@@ -68,7 +68,7 @@ def test_norm_refuses(over, words):
 
 @pytest.mark.parametrize('over, words, code', [
     (dict(dtype=1), 'dtype', INVALID), (dict(m=-1), 'size', INVALID), (dict(n=0), 'size', INVALID), (dict(k=0), 'size', INVALID),
-    (dict(k=131072), '131071', TOO_LARGE), (dict(m=65535 * 64 + 1), 'exceeds', TOO_LARGE), (dict(a=None), 'NULL', INVALID),
+    (dict(k=131072), '131071', TOO_LARGE), (dict(m=65535 * 64 + 1), 'exceeds', TOO_LARGE), (dict(n=65535 * 128 + 1, out_stride=2**24), 'exceeds', TOO_LARGE), (dict(a=None), 'NULL', INVALID),
     (dict(w_scales=None), 'NULL', INVALID), (dict(out=None), 'NULL', INVALID), (dict(out=BASE + 1), 'whole element', INVALID),
     (dict(bias=BASE + 2), 'whole element', INVALID), (dict(a_stride=15), 'strides', INVALID), (dict(out_stride=7), 'strides', INVALID)])
 def test_matmul_refuses(over, words, code):
