@@ -16,7 +16,8 @@ namespace n2d2b {
 static constexpr int PR_THREADS = 512, PR_BLOCK = 128, PR_CONSTS = 4;
 template <int D> struct PromptSmem {
     static constexpr int TILE = 128 * D * 2;                 // 128 rows (or tokens) of halves, in blocks of 64 columns
-    static constexpr int Q = 0, K = Q + 2 * TILE, V = K + 2 * TILE, BYTES = V + 2 * TILE + 1024;
+    static constexpr int Q = 0, K = Q + 2 * TILE, V = K + 2 * TILE, NEED = V + 2 * TILE + 1024;
+    static constexpr int BYTES = NEED > 227 * 1024 - 4096 ? NEED : 227 * 1024 - 4096;   // all of TMEM: a multiprocessor to itself
     static constexpr int PITCH = D + 4;                      // floats of a row of a part, in the tiles' place at the end
     static_assert(256 * PITCH * 4 <= 6 * TILE, "a part fits");
 };
@@ -79,7 +80,6 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_attention_prompt_kernel(cons
     __shared__ float part_top[256], part_sum[256];
     __shared__ unsigned tmem_slot;
     __shared__ int abort_flag;
-    pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
@@ -97,6 +97,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_attention_prompt_kernel(cons
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
+        pdl_wait();         // (see TMEM_BYTES)
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -104,6 +105,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_attention_prompt_kernel(cons
     __syncthreads();
     tc_fence_after();
     const unsigned tmem = tmem_slot;
+    pdl_launch_dependents();
     pdl_wait();
 
     // the rows with the most to see come first

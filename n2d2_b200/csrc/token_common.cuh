@@ -67,6 +67,11 @@ static inline cudaError_t launch_token(void (*kernel)(P...), dim3 grid, int thre
 }
 
 // ----------------------------------------------------------------------------- clusters
+// TMEM is handed out at run time, and a block that waits for its share while blocks that hold theirs wait for it would wait for ever.
+// Three rules keep that from happening: a block asks for at least this much shared memory for each TMEM column (the multiprocessor's
+// 228 KB over 512 columns, rounded up), so whatever blocks of these kernels share a multiprocessor, their columns fit; it allocates
+// behind griddepcontrol.wait, so it never holds columns that the kernel before it still needs; and it lets the next kernel start only then.
+static constexpr int TMEM_BYTES = 460;
 __device__ __forceinline__ unsigned cluster_rank()
 {
     unsigned r;

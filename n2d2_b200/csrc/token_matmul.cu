@@ -67,7 +67,6 @@ __global__ void __launch_bounds__(192, 1) matmul_i8_tile_kernel(const __grid_con
     __shared__ unsigned tmem_slot;
     __shared__ int abort_flag;
     __shared__ float sa[COLUMNS];
-    pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         if (!BYTES) { prefetch_tensor_map(&w_map); prefetch_tensor_map(&a_map); }
@@ -77,6 +76,7 @@ __global__ void __launch_bounds__(192, 1) matmul_i8_tile_kernel(const __grid_con
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
+        pdl_wait();         // (see TMEM_BYTES)
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"((unsigned)COLUMNS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -84,6 +84,7 @@ __global__ void __launch_bounds__(192, 1) matmul_i8_tile_kernel(const __grid_con
     __syncthreads();
     tc_fence_after();
     const unsigned tmem = tmem_slot;
+    pdl_launch_dependents();
     pdl_wait();
 
     const unsigned rank = cluster_rank(), ranks = cluster_size();
@@ -245,7 +246,6 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) matmul_i8_pair_kernel(const _
     __shared__ __align__(8) unsigned long long full[PAIR_STAGES], empty[PAIR_STAGES], tfull[2], tempty[2];
     __shared__ unsigned tmem_slot;
     __shared__ int abort_flag;
-    pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const unsigned rank = cluster_rank();
     if (threadIdx.x == 0) {
@@ -257,6 +257,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) matmul_i8_pair_kernel(const _
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
+        pdl_wait();
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
@@ -265,6 +266,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) matmul_i8_pair_kernel(const _
     cluster_sync();
     tc_fence_after();
     const unsigned tmem = tmem_slot;
+    pdl_launch_dependents();
     pdl_wait();
 
     const int blocks = (p.K + MM_K - 1) / MM_K;
@@ -360,7 +362,7 @@ static cudaError_t launch_tile(const MatmulArgs& p, int split, int* status, cuda
     stages = stages < room ? stages : room;
     stages = stages < 12 ? stages : 12;
     const int part = split > 1 ? BN * 128 * 4 : 0;
-    const int bytes = (stages * STAGE > part ? stages * STAGE : part) + 1024;
+    const int need = (stages * STAGE > part ? stages * STAGE : part) + 1024, least = (BN < 32 ? 32 : BN) * TMEM_BYTES, bytes = need > least ? need : least;
     const cudaError_t e = raise_smem_limit(matmul_i8_tile_kernel<T, BN, BYTES>, set, TILE_RING + 1024);
     if (e != cudaSuccess) return e;
     const dim3 grid((unsigned)split, (unsigned)((p.N + 127) / 128), (unsigned)((p.M + BN - 1) / BN));
