@@ -1,19 +1,20 @@
 // Attention of many new tokens over the paged 8-bit cache, on the tensor cores (the mathematics: kv_attention.cu).
 //
 // A block takes 256 rows (new token x query head of one key head, two tiles of 128) and walks over the tokens they see, 128 at a time.
-//   warps 4-7    bring pages through registers and write their codes as halves (exact) where the MMAs read them, swizzled
 //   warp 0       issues the MMAs: S = Q K^T (128 x 128, 32-bit sums in TMEM), O += P V with P read from TMEM in S's place
-//   warps 8-15   a thread holds one row of one tile: scores to probabilities, running maximum and sum, at the end O / sum
-// While the tensor pipe works on one tile, the other tile's rows are in the hands of their threads.  The output is only rescaled when a row's
-// maximum has grown by more than 2^8: below that the probabilities stay far inside 16 bits and their sum in 32 whatever the maximum they are
-// taken against.
+//   warp 1       the scales of the pages
+//   warps 4-7    bring keys through registers and write their codes as halves (exact) where the MMAs read them, swizzled; 8-11 the same for values
+//   warps 12-19  a thread holds one row of one tile: scores to probabilities, running maximum and sum, at the end O / sum
+// While the tensor pipe works on one tile, the other tile's rows are in the hands of their threads, 32 scores at a time with the next 32 on
+// their way.  A row's maximum only moves, and the output so far is only rescaled, when a score is more than 2^8 above it: below that the
+// probabilities stay far inside 16 bits and their sum in 32 whatever the maximum they are taken against.
 #include <cstdio>
 #include <cstring>
 #include "kv_common.cuh"
 
 namespace n2d2b {
 
-static constexpr int PR_THREADS = 512, PR_BLOCK = 128, PR_CONSTS = 4;
+static constexpr int PR_THREADS = 640, PR_BLOCK = 128, PR_CONSTS = 4;
 template <int D> struct PromptSmem {
     static constexpr int TILE = 128 * D * 2;                 // 128 rows (or tokens) of halves, in blocks of 64 columns
     static constexpr int Q = 0, K = Q + 2 * TILE, V = K + 2 * TILE, NEED = V + 2 * TILE + 1024;
@@ -41,20 +42,17 @@ __device__ __forceinline__ void tc_mma_f16_ts(unsigned d_tmem, unsigned a_tmem, 
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}"
         ::"r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate) : "memory");
 }
-__device__ __forceinline__ void tc_st8(unsigned taddr, const unsigned* v)
+__device__ __forceinline__ void tc_ld16(unsigned taddr, unsigned* v)
 {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-                 ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+                   "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]) : "r"(taddr) : "memory");
 }
-__device__ __forceinline__ void tc_st32(unsigned taddr, const unsigned* v)
+__device__ __forceinline__ void tc_st16(unsigned taddr, const unsigned* v)
 {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
-        ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
-        "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]),
-        "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]) : "memory");
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+                 "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]));     // (no memory clobber: loads may pass it)
 }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void sts128(unsigned addr, unsigned x, unsigned y, unsigned z, unsigned w)
@@ -67,7 +65,7 @@ template <int N> __device__ __forceinline__ void fewer_registers() { asm volatil
 template <bool M> struct Masked { static constexpr bool value = M; };
 
 struct PromptBars {
-    unsigned long long k_full[2], k_empty[2], v_full[2], v_empty[2], q_full[2], s_full[2], p_full[2], o_full[2], c_full[PR_CONSTS];
+    unsigned long long k_full[2], k_empty[2], v_full[2], v_empty[2], q_full[2], s_full[2], p_full[2], o_full[2], c_full[PR_CONSTS], c_empty[PR_CONSTS];
 };
 
 template <typename T, int D>
@@ -92,7 +90,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_attention_prompt_kernel(cons
             mbar_init(smem_u32(&bars.s_full[i]), 1);
             mbar_init(smem_u32(&bars.o_full[i]), 1);
         }
-        for (int i = 0; i < PR_CONSTS; ++i) mbar_init(smem_u32(&bars.c_full[i]), 1);
+        for (int i = 0; i < PR_CONSTS; ++i) { mbar_init(smem_u32(&bars.c_full[i]), 1); mbar_init(smem_u32(&bars.c_empty[i]), 8); }
         abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -130,7 +128,34 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_attention_prompt_kernel(cons
 
     if (warp < 4) {
         fewer_registers<40>();
-        if (warp == 0 && blocks > 0) {
+        if (warp == 1) {
+            // lane i: scales of tokens 16 i .. 16 i + 15 of a block, ahead of the keys
+            auto number_of = [&](int j) -> int {
+                const int token = (j_lo + j) * PR_BLOCK + lane * 16;
+                return lane < 8 && j < blocks && token < hi ? a.c.table[(size_t)b * a.c.row + (token >> a.log_page)] : 0;
+            };
+            float k_scale = 0.0f, v_scale = 0.0f;
+            bool bad = false;
+            auto turn_to = [&](int page_number) {
+                bad = (unsigned)page_number >= (unsigned)a.c.nb_pages;
+                const int at = (bad ? 0 : page_number) * a.c.heads + head;
+                k_scale = a.c.k_scales[at];
+                v_scale = a.c.v_scales[at];
+            };
+            if (blocks > 0) turn_to(number_of(0));
+            int number = number_of(1);
+            for (int j = 0; j < blocks; ++j) {
+                if (j >= PR_CONSTS && !mbar_wait_issuer(smem_u32(&bars.c_empty[j & (PR_CONSTS - 1)]), (unsigned)(j / PR_CONSTS - 1) & 1u, &abort_flag, a.status, 46)) break;
+                if (lane < 8) {
+                    const float scale = v_scale <= TOKEN_TINY ? TOKEN_TINY : v_scale, log = __log2f(scale);       // (all codes are 0 there)
+                    consts[j & (PR_CONSTS - 1)][lane] = make_float4(bad ? __int_as_float(0x7fffffff) : k_scale, log, exp2_approx(-log), 0.0f);
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&bars.c_full[j & (PR_CONSTS - 1)]));
+                if (j + 1 < blocks) turn_to(number);
+                number = number_of(j + 2);
+            }
+        } else if (warp == 0 && blocks > 0) {
             const unsigned hi_k = (unsigned)(make_smem_desc(0u, 128) >> 32);
             const unsigned idesc_s = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
             const unsigned idesc_o = (1u << 4) | (1u << 16) | (((unsigned)D >> 3) << 17) | ((128u >> 4) << 24);   // values: tokens are rows
@@ -177,75 +202,57 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_attention_prompt_kernel(cons
                 }
             }
         }
-    } else if (warp < 8) {
-        fewer_registers<104>();
-        const int tid = threadIdx.x - 128;
+    } else if (warp < 12) {
+        fewer_registers<88>();
+        const bool keys = warp < 8;
+        const int tid = (threadIdx.x - 128) & 127;
         constexpr int CHUNKS = D / 16, ROWS = 128 / CHUNKS, PASSES = 128 / ROWS;   // 16 codes a chunk, tokens of a pass, passes of a block
-        const int row = tid / CHUNKS, chunk = tid % CHUNKS;
-        PageOf held;        // lane i: tokens 16 i .. 16 i + 15 of the next block
-        auto fetch = [&](int j) {
+        // eight lanes write two rows' halves of a 64-column block: no two on one bank
+        const int row = CHUNKS == 8 ? (tid >> 5) * 4 + ((tid >> 4) & 1) * 2 + ((tid >> 2) & 1) : tid / CHUNKS;
+        const int chunk = CHUNKS == 8 ? ((tid >> 3) & 1) * 4 + (tid & 3) : tid % CHUNKS;
+        const int8_t* const from = (keys ? a.c.k : a.c.v) + chunk * 16;
+        // lane i: page number of tokens 16 i .. 16 i + 15 of a block, asked for two blocks ahead
+        auto number_of = [&](int j) -> int {
             const int token = (j_lo + j) * PR_BLOCK + lane * 16;
-            held = page_of(a.c, b, head, token >> a.log_page, lane < 8 && j < blocks && token < hi);
+            return lane < 8 && j < blocks && token < hi ? a.c.table[(size_t)b * a.c.row + (token >> a.log_page)] : 0;
         };
-        auto load = [&](uint4* r, const int8_t* from) {
+        uint4 x[PASSES];
+        auto load = [&](int number) {
+            const int first = (((unsigned)number < (unsigned)a.c.nb_pages ? number : 0) * a.c.heads + head) << a.log_page;
 #pragma unroll
             for (int i = 0; i < PASSES; ++i) {
                 const int t = i * ROWS + row;          // token of the block
-                const int number = __shfl_sync(0xffffffffu, held.number, t >> 4);
-                const int place = t & ((1 << a.log_page) - 1);
-                const size_t line = (((size_t)number * a.c.heads + head) << a.log_page) + (size_t)place;
-                r[i] = *reinterpret_cast<const uint4*>(from + line * D + chunk * 16);
+                const int line = __shfl_sync(0xffffffffu, first, t >> 4) + (t & ((1 << a.log_page) - 1));
+                x[i] = *reinterpret_cast<const uint4*>(from + (size_t)(unsigned)line * D);
             }
         };
-        // chunk of 16 halves pairs inside a row's 64-column block; lanes of the second block write in the other order: no two on one bank
-        const unsigned flip = (unsigned)(chunk >> 2) & 1u;
-        auto store = [&](const uint4* r, unsigned at) {
+        const unsigned full = smem_u32(keys ? bars.k_full : bars.v_full), empty = smem_u32(keys ? bars.k_empty : bars.v_empty);
+        const unsigned to = base + (keys ? S::K : S::V) + (unsigned)((chunk >> 2) * 16384 + row * 128);
+        if (blocks > 0) load(number_of(0));
+        int number = number_of(1);
+        for (int j = 0; j < blocks; ++j) {
+            if (j >= 2 && !mbar_wait_warp(empty + 8u * (j & 1), (unsigned)((j >> 1) - 1) & 1u, &abort_flag, a.status, 45)) break;
 #pragma unroll
             for (int i = 0; i < PASSES; ++i) {
-                const int t = i * ROWS + row;
-                const unsigned w[4] = {r[i].x ^ 0x80808080u, r[i].y ^ 0x80808080u, r[i].z ^ 0x80808080u, r[i].w ^ 0x80808080u};
+                const unsigned w[4] = {x[i].x ^ 0x80808080u, x[i].y ^ 0x80808080u, x[i].z ^ 0x80808080u, x[i].w ^ 0x80808080u};
                 unsigned h[8];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) { h[2 * e] = less_1152(splice(w[e], 0x4140)); h[2 * e + 1] = less_1152(splice(w[e], 0x4342)); }
-                const unsigned line = at + (unsigned)((chunk >> 2) * 16384 + t * 128);
-                const unsigned c0 = (((unsigned)(chunk & 3) * 2 + flip) ^ (unsigned)(t & 7)) << 4, c1 = (((unsigned)(chunk & 3) * 2 + 1 - flip) ^ (unsigned)(t & 7)) << 4;
-                sts128(line + c0, flip ? h[4] : h[0], flip ? h[5] : h[1], flip ? h[6] : h[2], flip ? h[7] : h[3]);
-                sts128(line + c1, flip ? h[0] : h[4], flip ? h[1] : h[5], flip ? h[2] : h[6], flip ? h[3] : h[7]);
+                const unsigned line = to + (unsigned)((j & 1) * S::TILE + i * ROWS * 128), c = (((unsigned)(chunk & 3) * 2) ^ (unsigned)((i * ROWS + row) & 7)) << 4;
+                sts128(line + c, h[0], h[1], h[2], h[3]);
+                sts128(line + (c ^ 16u), h[4], h[5], h[6], h[7]);
             }
-        };
-        uint4 k[PASSES], v[PASSES];
-        bool ok = true;
-        if (blocks > 0) {
-            fetch(0);
-            load(k, a.c.k);
-            load(v, a.c.v);
-        }
-        for (int j = 0; j < blocks && ok; ++j) {
-            // (the scores of block j - 2 came behind the probabilities of block j - 3: nobody reads the constants of block j - 4 any more)
-            if (j >= 2) ok = mbar_wait_warp(smem_u32(&bars.k_empty[j & 1]), (unsigned)((j >> 1) - 1) & 1u, &abort_flag, a.status, 45);
-            if (!ok) break;
-            if (warp == 4 && lane < 8) consts[j & (PR_CONSTS - 1)][lane] = make_float4(held.k_scale, held.v_log, held.v_inverse, 0.0f);
-            if (warp == 4) {
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&bars.c_full[j & (PR_CONSTS - 1)]));
-            }
-            store(k, base + S::K + (unsigned)((j & 1) * S::TILE));
             fence_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&bars.k_full[j & 1]));
-            fetch(j + 1);
-            if (j + 1 < blocks) load(k, a.c.k);
-            if (j >= 2) ok = mbar_wait_warp(smem_u32(&bars.v_empty[j & 1]), (unsigned)((j >> 1) - 1) & 1u, &abort_flag, a.status, 46);
-            if (!ok) break;
-            store(v, base + S::V + (unsigned)((j & 1) * S::TILE));
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&bars.v_full[j & 1]));
-            if (j + 1 < blocks) load(v, a.c.v);
+            if (lane == 0) mbar_arrive(full + 8u * (j & 1));
+            if (j + 1 < blocks) {
+                load(number);
+                number = number_of(j + 2);
+            }
         }
     } else {
-        more_registers<184>();
-        const int i = (warp - 8) >> 2, r = threadIdx.x - 256 - i * 128;      // tile and row
+        more_registers<128>();
+        const int i = (warp - 12) >> 2, r = threadIdx.x - 384 - i * 128;     // tile and row
         const int row = row0 + i * 128 + r, t = row / a.group, h = row - t * a.group;
         const bool there = row < s.count * a.group;
         const int pos = s.begin + t;
@@ -256,18 +263,14 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_attention_prompt_kernel(cons
         }
         float sum = there && see_hi > capacity ? __int_as_float(0x7fffffff) : 0.0f, top = -INFINITY, row_scale = 0.0f;
         if (blocks > 0 && (i == 0 || two)) {
-            uint4 w[D / 8];
             const T* const q = (const T*)a.q + (size_t)(s.first_row + t) * a.q_stride + (size_t)(head * a.group + h) * D;
-#pragma unroll
-            for (int e = 0; e < D / 8; ++e) {
-                w[e] = make_uint4(0, 0, 0, 0);
-                if (there) w[e] = *reinterpret_cast<const uint4*>(q + 8 * e);
-            }
             unsigned largest = 0;
-#pragma unroll
+#pragma unroll 4
             for (int e = 0; e < D / 8; ++e) {
+                uint4 w = make_uint4(0, 0, 0, 0);
+                if (there) w = *reinterpret_cast<const uint4*>(q + 8 * e);
                 float f[8];
-                Elem<T>::unpack(w[e], f);
+                Elem<T>::unpack(w, f);
 #pragma unroll
                 for (int x = 0; x < 8; ++x) largest = max(largest, magnitude(f[x]));
             }
@@ -276,10 +279,12 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_attention_prompt_kernel(cons
             const bool scaled = exponent > 0 && largest < 0x7f800000u;
             const float up = copysignf(scaled ? __int_as_float((254 - exponent) << 23) : 1.0f, a.scale_log2);
             row_scale = fabsf(a.scale_log2) * (scaled ? __int_as_float(exponent << 23) : 1.0f);
-#pragma unroll
+#pragma unroll 4
             for (int e = 0; e < D / 8; ++e) {
+                uint4 w = make_uint4(0, 0, 0, 0);
+                if (there) w = *reinterpret_cast<const uint4*>(q + 8 * e);
                 float f[8];
-                Elem<T>::unpack(w[e], f);
+                Elem<T>::unpack(w, f);
                 sts128(base + S::Q + (unsigned)(i * S::TILE + (e >> 3) * 16384 + r * 128 + (((e & 7) ^ (r & 7)) << 4)), pack_half2(f[0] * up, f[1] * up),
                        pack_half2(f[2] * up, f[3] * up), pack_half2(f[4] * up, f[5] * up), pack_half2(f[6] * up, f[7] * up));
             }
@@ -290,62 +295,81 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_attention_prompt_kernel(cons
         const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
         const unsigned s_at = tmem + lanes + (unsigned)(i * 128), o_at = tmem + lanes + 256u + (unsigned)(i * 128);
         bool ok = true;
-        if (i == 0 || two) {
+        if (i == 1 && !two) {
+            for (int j = 0; j < blocks; ++j) {      // a tile without rows: only hands the constants on
+                if (!mbar_wait_issuer(smem_u32(&bars.c_full[j & (PR_CONSTS - 1)]), (unsigned)(j / PR_CONSTS) & 1u, &abort_flag, a.status, 47)) break;
+                if (lane == 0) mbar_arrive(smem_u32(&bars.c_empty[j & (PR_CONSTS - 1)]));
+            }
+        } else {
             for (int j = 0; j < blocks; ++j) {
                 const int j0 = (j_lo + j) * PR_BLOCK;
                 ok = mbar_wait_warp(smem_u32(&bars.c_full[j & (PR_CONSTS - 1)]), (unsigned)(j / PR_CONSTS) & 1u, &abort_flag, a.status, 47)
                      && mbar_wait_warp(smem_u32(&bars.s_full[i]), (unsigned)j & 1u, &abort_flag, a.status, 48);
                 if (!ok) break;
                 tc_fence_after();
-                unsigned x[128];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tc_ld32(s_at + 32u * c, x + 32 * c);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tc_wait_ld_into(x + 32 * c);
                 const float4* const group = consts[j & (PR_CONSTS - 1)];
-                // what a row does not see becomes -inf (only where a row of the warp sees less than the whole block)
-                const bool whole = see_lo <= j0 && see_hi >= j0 + PR_BLOCK;
-                const bool all_whole = __all_sync(0xffffffffu, whole);
-                if (!all_whole) {
-                    const unsigned first = (unsigned)(see_lo - j0), span = (unsigned)max(see_hi - see_lo, 0);
+                const bool whole = __all_sync(0xffffffffu, see_lo <= j0 && see_hi >= j0 + PR_BLOCK);
+                const unsigned first = (unsigned)(see_lo - j0), span = (unsigned)max(see_hi - see_lo, 0);
+
+                // scores 32 q .. 32 q + 31 to probabilities
+                auto quarter = [&](const int q, unsigned* x, const float4* f, auto masked) {
+                    constexpr bool MASKED = decltype(masked)::value;
+                    if (MASKED) {       // what a row does not see becomes -inf
 #pragma unroll
-                    for (int c = 0; c < 128; ++c)
-                        if ((unsigned)c - first >= span) x[c] = 0xff800000u;
-                }
-                float best = top;
+                        for (int c = 0; c < 32; ++c)
+                            if ((unsigned)(32 * q + c) - first >= span) x[c] = 0xff800000u;
+                    }
+                    float best = -INFINITY;
 #pragma unroll
-                for (int g = 0; g < 8; ++g) {
-                    float m = __uint_as_float(x[16 * g]);
+                    for (int g = 0; g < 2; ++g) {
+                        float m[4];
 #pragma unroll
-                    for (int e = 1; e < 16; ++e) m = fmaxf(m, __uint_as_float(x[16 * g + e]));
-                    const float4 f = group[g];
-                    best = fmaxf(best, m == -INFINITY ? -INFINITY : fmaf(m, f.x * row_scale, f.y));
-                }
-                const bool grown = best > top + 8.0f || (top == -INFINITY && best > top);
-                if (__any_sync(0xffffffffu, grown)) {
-                    const float fade = grown ? exp2_approx(top - best) : 1.0f;
-                    if (grown) top = best;
-                    sum *= fade;
-                    if (j > 0) {
+                        for (int e = 0; e < 4; ++e)
+                            m[e] = fmaxf(fmaxf(__uint_as_float(x[16 * g + e]), __uint_as_float(x[16 * g + 4 + e])),
+                                         fmaxf(__uint_as_float(x[16 * g + 8 + e]), __uint_as_float(x[16 * g + 12 + e])));
+                        const float most = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+                        best = fmaxf(best, MASKED && most == -INFINITY ? -INFINITY : fmaf(most, f[g].x * row_scale, f[g].y));
+                    }
+                    const bool moves = best > top + 8.0f || (top == -INFINITY && best > top);       // (each row for itself: another row's numbers change nothing in it)
+                    if (__any_sync(0xffffffffu, moves)) {
+                        const float fade = moves ? exp2_approx(top - best) : 1.0f;
+                        if (moves) top = best;
+                        sum *= fade;
+                        const __half2 fade2 = __float2half2_rn(fade);
 #pragma unroll 1
-                        for (int c = 0; c < D; c += 32) {
-                            unsigned o[32];
-                            tc_ld32(o_at + (unsigned)c, o);
-                            tc_wait_ld_into(o);
+                        for (int c = 0; c < 16 * q; c += 16) {        // this block's probabilities so far
+                            unsigned p[16];
+                            tc_ld16(s_at + (unsigned)c, p);
+                            tc_wait_ld();
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fade);
-                            tc_st32(o_at + (unsigned)c, o);
+                            for (int e = 0; e < 16; ++e) {
+                                asm volatile("" : "+r"(p[e])::"memory");
+                                const __half2 h = __hmul2(*reinterpret_cast<__half2*>(&p[e]), fade2);
+                                p[e] = *reinterpret_cast<const unsigned*>(&h);
+                            }
+                            tc_st16(s_at + (unsigned)c, p);
+                        }
+                        if (j > 0) {
+#pragma unroll 1
+                            for (int c = 0; c < D; c += 16) {
+                                unsigned o[16];
+                                tc_ld16(o_at + (unsigned)c, o);
+                                tc_wait_ld();
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) {
+                                    asm volatile("" : "+r"(o[e])::"memory");
+                                    o[e] = __float_as_uint(__uint_as_float(o[e]) * fade);
+                                }
+                                tc_st16(o_at + (unsigned)c, o);
+                            }
                         }
                     }
-                }
-                const float from = top == -INFINITY ? 0.0f : top;
-                auto probabilities = [&](auto masked) {
+                    const float from = top == -INFINITY ? 0.0f : top;
+                    unsigned packed[16];
 #pragma unroll
-                    for (int g = 0; g < 8; ++g) {
-                        const float4 f = group[g];
-                        const float by = f.x * row_scale, add = f.y - from;
-                        float part = 0.0f;
-                        unsigned packed[8];
+                    for (int g = 0; g < 2; ++g) {
+                        const float by = f[g].x * row_scale, add = f[g].y - from;
+                        float part[2] = {0.0f, 0.0f};
 #pragma unroll
                         for (int e = 0; e < 16; e += 2) {
                             float p[2];
@@ -353,21 +377,45 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_attention_prompt_kernel(cons
                             for (int y = 0; y < 2; ++y) {
                                 const float v = __uint_as_float(x[16 * g + e + y]);
                                 p[y] = exp2_approx(fmaf(v, by, add));
-                                if (decltype(masked)::value) p[y] = v == -INFINITY ? 0.0f : p[y];   // (whatever the scales of a page it does not see)
+                                if (MASKED) p[y] = v == -INFINITY ? 0.0f : p[y];   // (whatever the scales of a page it does not see)
+                                part[y] += p[y];
                             }
-                            part += p[0] + p[1];
-                            packed[e >> 1] = pack_half2(p[0], p[1]);
+                            packed[8 * g + (e >> 1)] = pack_half2(p[0], p[1]);
                         }
-                        if (!decltype(masked)::value || part != 0.0f) sum = fmaf(part, f.z, sum);
-                        tc_st8(s_at + (unsigned)(8 * g), packed);
+                        const float both = part[0] + part[1];
+                        if (!MASKED || both != 0.0f) sum = fmaf(both, f[g].z, sum);
                     }
+                    tc_st16(s_at + (unsigned)(16 * q), packed);
                 };
-                if (all_whole) probabilities(Masked<false>());
-                else probabilities(Masked<true>());
+                auto block = [&](auto masked) {
+                    // (the probabilities of 32 scores take 16 columns: they never reach what is still on its way)
+                    unsigned xa[32], xb[32];
+                    float4 fa[2] = {group[0], group[1]}, fb[2];
+                    tc_ld32(s_at, xa);
+                    tc_wait_ld_into(xa);
+                    tc_ld32(s_at + 32u, xb);
+                    fb[0] = group[2]; fb[1] = group[3];
+                    quarter(0, xa, fa, masked);
+                    tc_wait_ld_into(xb);
+                    tc_ld32(s_at + 64u, xa);
+                    fa[0] = group[4]; fa[1] = group[5];
+                    quarter(1, xb, fb, masked);
+                    tc_wait_ld_into(xa);
+                    tc_ld32(s_at + 96u, xb);
+                    fb[0] = group[6]; fb[1] = group[7];
+                    quarter(2, xa, fa, masked);
+                    tc_wait_ld_into(xb);
+                    quarter(3, xb, fb, masked);
+                };
+                if (whole) block(Masked<false>());
+                else block(Masked<true>());
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&bars.p_full[i]));
+                if (lane == 0) {
+                    mbar_arrive(smem_u32(&bars.p_full[i]));
+                    mbar_arrive(smem_u32(&bars.c_empty[j & (PR_CONSTS - 1)]));
+                }
             }
             if (ok && blocks > 0) ok = mbar_wait_warp(smem_u32(&bars.o_full[i]), 0, &abort_flag, a.status, 49);
             if (ranks > 1) {

@@ -88,9 +88,6 @@ __device__ __forceinline__ unsigned less_1152(unsigned h)
     const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half(0x6480)));
     return *reinterpret_cast<const unsigned*>(&d);
 }
-// Codes in bytes 0 and 2 (1 and 3) of a word as two halves
-__device__ __forceinline__ unsigned widen_even(unsigned w) { return less_1152((w & 0x00ff00ffu) ^ 0x64806480u); }
-__device__ __forceinline__ unsigned widen_odd(unsigned w) { return less_1152(((w >> 8) & 0x00ff00ffu) ^ 0x64806480u); }
 __device__ __forceinline__ float exp2_approx(float x)
 {
     float y;
@@ -114,31 +111,6 @@ __device__ __forceinline__ float4 ld_cluster4(unsigned addr)
     asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
     return v;
 }
-// One page's number and scales for a lane's unit half; what no query may see has no scale
-struct PageOf {
-    int number;
-    float k_scale, v_log, v_inverse;
-};
-__device__ __forceinline__ PageOf page_of(const KvArgs& c, int b, int head, int page, bool wanted)
-{
-    PageOf r = {0, 0.0f, 0.0f, 0.0f};
-    if (wanted) {
-        const float none = __int_as_float(0x7fffffff);
-        const int number = page < c.row ? c.table[(size_t)b * c.row + page] : -1;
-        if (number < 0 || number >= c.nb_pages) {
-            r.k_scale = none;
-        } else {
-            r.number = number;
-            r.k_scale = c.k_scales[(size_t)number * c.heads + head];
-            float v = c.v_scales[(size_t)number * c.heads + head];
-            if (v <= TOKEN_TINY) v = TOKEN_TINY;       // all codes are 0 then; any scale does
-            r.v_log = __log2f(v);
-            r.v_inverse = exp2_approx(-r.v_log);
-        }
-    }
-    return r;
-}
-
 // Many rows of a key head on the tensor cores (kv_attention_prompt.cu)
 cudaError_t launch_attention_prompt(const AttendArgs& a, int head_size, bool half, int sequences, cudaStream_t s);
 
