@@ -14,7 +14,7 @@
 
 namespace n2d2b {
 
-static constexpr int PR_THREADS = 640, PR_BLOCK = 128, PR_CONSTS = 4;
+static constexpr int PR_THREADS = 640, PR_BLOCK = 128, PR_CONSTS = 4, PR_POLYNOMIAL = 6;
 template <int D> struct PromptSmem {
     static constexpr int TILE = 128 * D * 2;                 // 128 rows (or tokens) of halves, in blocks of 64 columns
     static constexpr int Q = 0, K = Q + 2 * TILE, V = K + 2 * TILE, NEED = V + 2 * TILE + 1024;
@@ -62,6 +62,55 @@ __device__ __forceinline__ void sts128(unsigned addr, unsigned x, unsigned y, un
 template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
+// Two 32-bit values to an instruction
+typedef unsigned long long Pair;
+__device__ __forceinline__ Pair pair_of(float a, float b)
+{
+    Pair r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 both_of(Pair p)
+{
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+    return r;
+}
+__device__ __forceinline__ Pair fma_pair(Pair a, Pair b, Pair c)
+{
+    Pair d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ Pair add_pair(Pair a, Pair b)
+{
+    Pair d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float max_of(float a, float b, float c)
+{
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// 2^x for x up to 8 without the exponential unit, which a quarter of the probabilities is kept from (it takes 8 cycles for a warp's 32 and would bound
+// the kernel): x = n + f with n whole, 2^f on [-1/2, 1/2] by the polynomial of degree 4 with the smallest relative error (2.6e-6, from an exchange
+// iteration), n added to its exponent.  Below 2^-126 the result is that.
+__device__ __forceinline__ Pair exp2_pair(Pair x)
+{
+    const float2 v = both_of(x);
+    x = pair_of(fmaxf(v.x, -126.0f), fmaxf(v.y, -126.0f));
+    const Pair r = add_pair(x, pair_of(12582912.0f, 12582912.0f));      // 1.5 * 2^23: n in the lowest bits
+    const Pair f = fma_pair(add_pair(r, pair_of(-12582912.0f, -12582912.0f)), pair_of(-1.0f, -1.0f), x);
+    Pair p = pair_of(0.009570102207362652f, 0.009570102207362652f);
+    p = fma_pair(p, f, pair_of(0.05591785907745361f, 0.05591785907745361f));
+    p = fma_pair(p, f, pair_of(0.240247443318367f, 0.240247443318367f));
+    p = fma_pair(p, f, pair_of(0.6931217908859253f, 0.6931217908859253f));
+    p = fma_pair(p, f, pair_of(0.9999992847442627f, 0.9999992847442627f));
+    const float2 y = both_of(p), n = both_of(r);
+    return pair_of(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(n.x) << 23)), __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(n.y) << 23)));
+}
 template <bool M> struct Masked { static constexpr bool value = M; };
 
 struct PromptBars {
@@ -322,12 +371,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_attention_prompt_kernel(cons
                     float best = -INFINITY;
 #pragma unroll
                     for (int g = 0; g < 2; ++g) {
-                        float m[4];
+                        float m[5];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            m[e] = fmaxf(fmaxf(__uint_as_float(x[16 * g + e]), __uint_as_float(x[16 * g + 4 + e])),
-                                         fmaxf(__uint_as_float(x[16 * g + 8 + e]), __uint_as_float(x[16 * g + 12 + e])));
-                        const float most = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+                        for (int e = 0; e < 5; ++e) m[e] = max_of(__uint_as_float(x[16 * g + 3 * e]), __uint_as_float(x[16 * g + 3 * e + 1]), __uint_as_float(x[16 * g + 3 * e + 2]));
+                        const float most = max_of(max_of(m[0], m[1], m[2]), max_of(m[3], m[4], __uint_as_float(x[16 * g + 15])), -INFINITY);
                         best = fmaxf(best, MASKED && most == -INFINITY ? -INFINITY : fmaf(most, f[g].x * row_scale, f[g].y));
                     }
                     const bool moves = best > top + 8.0f || (top == -INFINITY && best > top);       // (each row for itself: another row's numbers change nothing in it)
@@ -368,21 +415,28 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_attention_prompt_kernel(cons
                     unsigned packed[16];
 #pragma unroll
                     for (int g = 0; g < 2; ++g) {
-                        const float by = f[g].x * row_scale, add = f[g].y - from;
-                        float part[2] = {0.0f, 0.0f};
+                        const float one_by = f[g].x * row_scale, one_add = f[g].y - from;
+                        const Pair by = pair_of(one_by, one_by), add = pair_of(one_add, one_add);
+                        Pair part[2] = {pair_of(0.0f, 0.0f), pair_of(0.0f, 0.0f)};
 #pragma unroll
                         for (int e = 0; e < 16; e += 2) {
-                            float p[2];
-#pragma unroll
-                            for (int y = 0; y < 2; ++y) {
-                                const float v = __uint_as_float(x[16 * g + e + y]);
-                                p[y] = exp2_approx(fmaf(v, by, add));
-                                if (MASKED) p[y] = v == -INFINITY ? 0.0f : p[y];   // (whatever the scales of a page it does not see)
-                                part[y] += p[y];
+                            const float v0 = __uint_as_float(x[16 * g + e]), v1 = __uint_as_float(x[16 * g + e + 1]);
+                            Pair p = fma_pair(pair_of(v0, v1), by, add);
+                            if ((e & 6) == PR_POLYNOMIAL) p = exp2_pair(p);
+                            else {
+                                const float2 t = both_of(p);
+                                p = pair_of(exp2_approx(t.x), exp2_approx(t.y));
                             }
-                            packed[8 * g + (e >> 1)] = pack_half2(p[0], p[1]);
+                            float2 y = both_of(p);
+                            if (MASKED) {       // (whatever the scales of a page it does not see)
+                                y = make_float2(v0 == -INFINITY ? 0.0f : y.x, v1 == -INFINITY ? 0.0f : y.y);
+                                p = pair_of(y.x, y.y);
+                            }
+                            part[(e >> 1) & 1] = add_pair(part[(e >> 1) & 1], p);
+                            packed[8 * g + (e >> 1)] = pack_half2(y.x, y.y);
                         }
-                        const float both = part[0] + part[1];
+                        const float2 sums = both_of(add_pair(part[0], part[1]));
+                        const float both = sums.x + sums.y;
                         if (!MASKED || both != 0.0f) sum = fmaf(both, f[g].z, sum);
                     }
                     tc_st16(s_at + (unsigned)(16 * q), packed);
