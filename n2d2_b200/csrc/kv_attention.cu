@@ -455,14 +455,15 @@ template <typename T, int D, int R>
 static cudaError_t launch_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendArgs& a, int sequences, cudaStream_t s)
 {
     const long long rows = (long long)a.c.max_new * a.group, blocks = (rows + R - 1) / R * a.c.heads * sequences;
-    const long long most = a.window ? min((long long)a.c.row << a.log_page, (long long)a.window + a.c.max_new) : (long long)a.c.row << a.log_page;
-    const long long steps = (most + ROWS_BLOCK - 1) / ROWS_BLOCK + (a.window ? 1 : 0);
+    const long long steps = attend_steps(a);
     // Streams of tokens to a tile: as many as give each multiprocessor two, at least two blocks to a stream.  One stream of 128 x 128 codes takes about 1300
     // cycles a block, half of what a multiprocessor's share of the memory takes for two.  Measured (streams to a tile: us): 8 tiles of 65000 tokens 4: 93,
     // 8: 51, 16: 33; 32 tiles of 15800 (heads of 64) 4: 31, 8: 21, 16: 36; 128 tiles of 2000 1: 19.6, 2: 14.0, 4: 19.0; 384 tiles of 8000 and
     // fewer 1: 91, 2: 81, 4: 90.  Two streams share a block (14.0 and 81 us; as clusters of two blocks 14.8 and 84), more are clusters.
+    // Tiles of 16 rows have a multiprocessor to themselves (their share of TMEM takes 115 KB of shared memory).
     int streams = 1;
-    while (streams < 16 && (blocks * streams * 2 <= 2 * token_sms() || (streams == 1 && steps >= 16)) && streams * 2 * 2 <= steps) streams *= 2;
+    if (R == 16) streams = attend_streams(blocks, steps, 1, 16);
+    else while (streams < 16 && (blocks * streams * 2 <= 2 * token_sms() || (streams == 1 && steps >= 16)) && streams * 2 * 2 <= steps) streams *= 2;
     const int groups = R < 16 && streams == 2 ? 2 : 1, split = streams / groups;
     // (a slot is filled again two blocks later: three at least, unless there are no more blocks than slots)
     const long long per = (steps + split * groups - 1) / (split * groups);
@@ -486,15 +487,23 @@ template <> struct Half<__half> { static constexpr bool value = true; };
 template <typename T>
 static cudaError_t launch_attention(const n2d2b_kv_cache& cache, const AttendArgs& a, int sequences, cudaStream_t s)
 {
-    // from here on the tensor cores' tiles of 128 rows are filled well enough
-    if ((long long)a.c.max_new * a.group > 64 && sequences * (long long)a.c.heads * (((long long)a.c.max_new * a.group + 255) / 256) < (1ll << 27))
-        return launch_attention_prompt(a, cache.head_size, Half<T>::value, sequences, s);
+    // Tiles of 16 rows or of 256: a step of 128 tokens takes the former about 2000 cycles and one of the latter, as long as it is not full, 5000; 9000 and 15000
+    // go with a wave of blocks.  Measured (us, 16 rows a tile / 256): 8 x 8 new tokens of 4 heads over 4000 38 / 70, 1 x 12 over 20000 57 / 92,
+    // 32 x 16 over 600 57 / 40, 32 x 32 over 1000 133 / 60, 8 x 64 of one head over 64 15 / 9.
+    const long long rows = (long long)a.c.max_new * a.group, key_heads = (long long)sequences * a.c.heads, steps = attend_steps(a), sms = token_sms();
+    if (rows > 16) {
+        const long long few = (rows + 15) / 16 * key_heads, many = (rows + 255) / 256 * key_heads;
+        const long long few_streams = attend_streams(few, steps, 1, 16), many_streams = attend_streams(many, steps, 2, 8);
+        const long long few_cycles = (few * few_streams + sms - 1) / sms * ((steps + few_streams - 1) / few_streams * 2000 + 9000);
+        const long long many_cycles = (many * many_streams + sms - 1) / sms * ((steps + many_streams - 1) / many_streams * 5000 + 15000);
+        if (many_cycles < few_cycles && many < (1ll << 27)) return launch_attention_prompt(a, cache.head_size, Half<T>::value, sequences, s);
+    }
     CUtensorMap k_map, v_map;
-    const unsigned long long rows = (unsigned long long)cache.nb_pages * cache.nb_heads * cache.page_tokens;
+    const unsigned long long lines = (unsigned long long)cache.nb_pages * cache.nb_heads * cache.page_tokens;
     const unsigned box = cache.page_tokens;
     const CUtensorMapSwizzle swizzle = cache.head_size == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
-    if (!token_byte_map(&k_map, cache.k, cache.head_size, rows, cache.head_size, cache.head_size, box, swizzle)
-        || !token_byte_map(&v_map, cache.v, cache.head_size, rows, cache.head_size, cache.head_size, box, swizzle))
+    if (!token_byte_map(&k_map, cache.k, cache.head_size, lines, cache.head_size, cache.head_size, box, swizzle)
+        || !token_byte_map(&v_map, cache.v, cache.head_size, lines, cache.head_size, cache.head_size, box, swizzle))
         return cudaErrorInvalidValue;
     return cache.head_size == 64 ? launch_rows_by_count<T, 64>(k_map, v_map, a, sequences, s) : launch_rows_by_count<T, 128>(k_map, v_map, a, sequences, s);
 }

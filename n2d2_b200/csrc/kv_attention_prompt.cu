@@ -550,10 +550,8 @@ static cudaError_t launch_prompt_of(const AttendArgs& a, int sequences, cudaStre
     const cudaError_t e = raise_smem_limit(kv_attention_prompt_kernel<T, D>, set, PromptSmem<D>::BYTES);
     if (e != cudaSuccess) return e;
     const long long tiles = ((long long)a.c.max_new * a.group + 255) / 256, blocks = tiles * a.c.heads * sequences;
-    const long long most = a.window ? min((long long)a.c.row << a.log_page, (long long)a.window + a.c.max_new) : (long long)a.c.row << a.log_page;
     // where half of the multiprocessors would have nothing to do, clusters share the tokens, at least two steps to a block
-    int split = 1;
-    while (split < 8 && blocks * split * 2 <= token_sms() && split * 4 * PR_BLOCK <= most) split *= 2;
+    const int split = attend_streams(blocks, attend_steps(a), 2, 8);
     return launch_token(kv_attention_prompt_kernel<T, D>, dim3((unsigned)(blocks * split)), PR_THREADS, PromptSmem<D>::BYTES, split, s, a, (int)tiles, sequences);
 }
 

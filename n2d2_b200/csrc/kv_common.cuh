@@ -111,6 +111,20 @@ __device__ __forceinline__ float4 ld_cluster4(unsigned addr)
     asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
     return v;
 }
+// Steps of 128 tokens that a row may see
+static inline long long attend_steps(const AttendArgs& a)
+{
+    const long long capacity = (long long)a.c.row << a.log_page, most = a.window && (long long)a.window + a.c.max_new < capacity ? (long long)a.window + a.c.max_new : capacity;
+    return (most + 127) / 128 + (a.window ? 1 : 0);
+}
+// Streams that the tokens of a tile are cut into: as many as leave no two blocks on a multiprocessor, of at least `least` steps each
+static inline int attend_streams(long long tiles, long long steps, int least, int most)
+{
+    int streams = 1;
+    while (streams < most && tiles * streams * 2 <= token_sms() && streams * 2 * least <= steps) streams *= 2;
+    return streams;
+}
+
 // Many rows of a key head on the tensor cores (kv_attention_prompt.cu)
 cudaError_t launch_attention_prompt(const AttendArgs& a, int head_size, bool half, int sequences, cudaStream_t s);
 

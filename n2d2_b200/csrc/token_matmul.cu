@@ -28,12 +28,24 @@ static constexpr int MM_K = 128, TILE_RING = 200 * 1024;
 template <typename T>
 __device__ __forceinline__ void store_columns(const MatmulArgs& p, const unsigned* acc, const float* sa, int token, int left, int channel, float sw, float bias)
 {
-    if (channel >= p.N) return;
     T* out = (T*)p.out + (size_t)token * p.out_stride + channel;
+    const bool there = channel < p.N;
+    // eight at a time: their arithmetic first, then their stores (a value and its store in turn took 60 cycles a column, this takes 25; all 32 at
+    // once no less, and their registers keep other blocks off the multiprocessor)
 #pragma unroll
-    for (int c = 0; c < 32; ++c) {
-        if (c < left) *out = Elem<T>::from_float(fmaf((float)(int)acc[c] * sa[c], sw, bias));
-        out += p.out_stride;
+    for (int c = 0; c < 32; c += 8) {
+        T v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = Elem<T>::from_float(fmaf((float)(int)acc[c + e] * sa[c + e], sw, bias));
+        if (there && c + 8 <= left) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) out[(long long)e * p.out_stride] = v[e];
+        } else if (there) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (c + e < left) out[(long long)e * p.out_stride] = v[e];
+        }
+        out += 8 * p.out_stride;
     }
 }
 
@@ -347,6 +359,14 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) matmul_i8_pair_kernel(const _
     }
 }
 
+// Blocks that share a multiprocessor so that all of a call run at once, four at most (their rings get the smaller for it)
+static int tile_residents(const MatmulArgs& p, int sms, int bn, int split)
+{
+    const long long ctas = (long long)((p.N + 127) / 128) * ((p.M + bn - 1) / bn) * split, each = (ctas + sms - 1) / sms;
+    const int most = bn >= 256 ? 1 : bn == 128 ? 2 : 4;
+    return each < most ? (int)each : most;
+}
+
 template <typename T, int BN, bool BYTES>
 static cudaError_t launch_tile(const MatmulArgs& p, int split, int* status, cudaStream_t s)
 {
@@ -357,7 +377,7 @@ static cudaError_t launch_tile(const MatmulArgs& p, int split, int* status, cuda
         || !token_byte_map(&a_map, p.a, p.K, p.M, p.a_stride, MM_K, BN, CU_TENSOR_MAP_SWIZZLE_128B))
         return cudaErrorInvalidValue;
     constexpr int STAGE = (128 + BN) * MM_K;
-    const int blocks = (p.K + MM_K - 1) / MM_K, room = TILE_RING / STAGE;
+    const int blocks = (p.K + MM_K - 1) / MM_K, room = TILE_RING / tile_residents(p, token_sms(), BN, split) / STAGE;
     int stages = (blocks + split - 1) / split;
     stages = stages < room ? stages : room;
     stages = stages < 12 ? stages : 12;
@@ -384,18 +404,22 @@ static cudaError_t launch_pair(const MatmulArgs& p, int sms, int* status, cudaSt
     return launch_token(matmul_i8_pair_kernel<T>, dim3((unsigned)(2 * pairs)), PAIR_THREADS, PAIR_SMEM, 2, s, w_map, a_map, p, tiles_n, tiles, status);
 }
 
-// Cycles that a call is expected to take, by the number of tokens of a tile and of blocks that share one (0 tokens: pairs)
-static long long expected_cycles(const MatmulArgs& p, int sms, int bn, int split, bool bytes)
+// Cycles that a call is expected to take, by the number of tokens of a tile and of blocks that share one (0 tokens: pairs).  The constants are fitted to
+// a sweep of both over 25 shapes from 1 x 4096 x 4096 to 4096 x 4096 x 4096: what it chooses takes 0.1 % longer than the best on average, 6 % at
+// most (150 x 1000 x 8000); the other choices take up to four times as long.
+static double expected_cycles(const MatmulArgs& p, int sms, int bn, int split, bool bytes)
 {
-    const long long blocks = (p.K + MM_K - 1) / MM_K;
+    const double blocks = (p.K + MM_K - 1) / MM_K;
     if (bn == 0) {
         const long long tiles = (long long)((p.N + 255) / 256) * ((p.M + 255) / 256), waves = (tiles + sms / 2 - 1) / (sms / 2);
-        return waves * blocks * 512 + 6000;
+        return 5000 + waves * (blocks * 705 > 7400 ? blocks * 705 : 7400);     // (a tile's stores run beside the next one's products)
     }
-    const long long ctas = (long long)((p.N + 127) / 128) * ((p.M + bn - 1) / bn) * split, waves = (ctas + sms - 1) / sms;
-    // a step's MMAs (128 cycles for 256 tokens, no fewer than 50), or its bytes at 71 a cycle (through registers: 16)
-    const long long mma = bn >= 128 ? bn * 2 : 200, load = (128 + bn) * MM_K / (bytes ? 16 : 71);
-    return waves * ((blocks + split - 1) / split * (mma > load ? mma : load) + 3500 + bn * 8) + (split > 1 ? 1200 + bn * 12 : 0);
+    const long long ctas = (long long)((p.N + 127) / 128) * ((p.M + bn - 1) / bn) * split, each = (ctas + sms - 1) / sms;
+    if (split == 8 && each > 1) return 1e30;       // (clusters of eight find no place beside one another: 14.4 us instead of 9.7 for 48 x 6144 x 4096)
+    const long long residents = tile_residents(p, sms, bn, split), rounds = (each + residents - 1) / residents;
+    // a step's MMAs (128 cycles for 256 tokens, no fewer than 50 an MMA), or its bytes at 45 a cycle (through registers: 12)
+    const double mma = bn >= 128 ? bn * 2 : 200, load = (128 + bn) * MM_K / (bytes ? 12.0 : 45.0), share = ctas > sms ? (double)ctas / sms : 1.0;
+    return 3000 + share * (((p.K + MM_K - 1) / MM_K + split - 1) / split) * (mma > load ? mma : load) + rounds * (1050 + bn * 9.0) + (split > 1 ? 2700 + bn * (26 + 0.4 * split) : 0.0);
 }
 
 template <typename T, bool BYTES>
@@ -418,11 +442,11 @@ static cudaError_t launch_matmul(const MatmulArgs& p, cudaStream_t s)
     if (!status) return cudaErrorInvalidSymbol;
     const int sms = token_sms(), blocks = (p.K + MM_K - 1) / MM_K;
     int best_bn = 0, best_split = 1;
-    long long best = p.M > 128 && !bytes ? expected_cycles(p, sms, 0, 1, false) : 1ll << 62;
+    double best = bytes ? 1e30 : expected_cycles(p, sms, 0, 1, false);
     for (int bn = 16; bn <= 256; bn *= 2) {
         if ((p.M + bn - 1) / bn > 65535) continue;
         for (int split = 1; split <= 8 && split <= blocks; split *= 2) {
-            const long long c = expected_cycles(p, sms, bn, split, bytes);
+            const double c = expected_cycles(p, sms, bn, split, bytes);
             if (c < best) { best = c; best_bn = bn; best_split = split; }
         }
         if (bn >= p.M) break;
