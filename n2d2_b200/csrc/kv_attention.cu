@@ -460,9 +460,10 @@ static cudaError_t launch_rows(const CUtensorMap& k_map, const CUtensorMap& v_ma
     // cycles a block, half of what a multiprocessor's share of the memory takes for two.  Measured (streams to a tile: us): 8 tiles of 65000 tokens 4: 93,
     // 8: 51, 16: 33; 32 tiles of 15800 (heads of 64) 4: 31, 8: 21, 16: 36; 128 tiles of 2000 1: 19.6, 2: 14.0, 4: 19.0; 384 tiles of 8000 and
     // fewer 1: 91, 2: 81, 4: 90.  Two streams share a block (14.0 and 81 us; as clusters of two blocks 14.8 and 84), more are clusters.
-    // Tiles of 16 rows have a multiprocessor to themselves (their share of TMEM takes 115 KB of shared memory).
+    // Tiles of 16 rows have a multiprocessor to themselves (their share of TMEM takes 115 KB of shared memory); sixteen such neighbours are hard to come
+    // by: 8 tiles of 4000 tokens 22.6 us as clusters of 16, 13.1 as clusters of 8.
     int streams = 1;
-    if (R == 16) streams = attend_streams(blocks, steps, 1, 16);
+    if (R == 16) streams = attend_streams(blocks, steps, 1, 8);
     else while (streams < 16 && (blocks * streams * 2 <= 2 * token_sms() || (streams == 1 && steps >= 16)) && streams * 2 * 2 <= steps) streams *= 2;
     const int groups = R < 16 && streams == 2 ? 2 : 1, split = streams / groups;
     // (a slot is filled again two blocks later: three at least, unless there are no more blocks than slots)
@@ -487,15 +488,17 @@ template <> struct Half<__half> { static constexpr bool value = true; };
 template <typename T>
 static cudaError_t launch_attention(const n2d2b_kv_cache& cache, const AttendArgs& a, int sequences, cudaStream_t s)
 {
-    // Tiles of 16 rows or of 256: a step of 128 tokens takes the former about 2000 cycles and one of the latter, as long as it is not full, 5000; 9000 and 15000
-    // go with a wave of blocks.  Measured (us, 16 rows a tile / 256): 8 x 8 new tokens of 4 heads over 4000 38 / 70, 1 x 12 over 20000 57 / 92,
-    // 32 x 16 over 600 57 / 40, 32 x 32 over 1000 133 / 60, 8 x 64 of one head over 64 15 / 9.
-    const long long rows = (long long)a.c.max_new * a.group, key_heads = (long long)sequences * a.c.heads, steps = attend_steps(a), sms = token_sms();
+    // Tiles of 16 rows or of 256: a step of 128 tokens takes the former about 2000 cycles and the latter 5000 (7000 with one of its halves empty, which
+    // then waits for its own products); 12000 and 15000 go with the blocks themselves.  Measured (us, 16 rows a tile / 256): 8 sequences of 8 new tokens of 4
+    // heads over 4000 38 / 70, 1 of 12 over 20000 50 / 92, 8 of 12 over 4000 44 / 66, 32 of 16 over 600 57 / 40, 32 of 32 over 1000 133 / 60, 8 of 64 of one
+    // head over 64 15 / 9.
+    const long long rows = (long long)a.c.max_new * a.group, key_heads = (long long)sequences * a.c.heads, steps = attend_steps(a);
     if (rows > 16) {
         const long long few = (rows + 15) / 16 * key_heads, many = (rows + 255) / 256 * key_heads;
-        const long long few_streams = attend_streams(few, steps, 1, 16), many_streams = attend_streams(many, steps, 2, 8);
-        const long long few_cycles = (few * few_streams + sms - 1) / sms * ((steps + few_streams - 1) / few_streams * 2000 + 9000);
-        const long long many_cycles = (many * many_streams + sms - 1) / sms * ((steps + many_streams - 1) / many_streams * 5000 + 15000);
+        const int few_streams = attend_streams(few, steps, 1, 8), many_streams = attend_streams(many, steps, 2, 8);
+        const double sms = token_sms(), few_waves = few * few_streams / sms, many_waves = many * many_streams / sms;
+        const double few_cycles = (few_waves > 1 ? few_waves : 1) * ((steps + few_streams - 1) / few_streams * 2000.0 + 12000);
+        const double many_cycles = (many_waves > 1 ? many_waves : 1) * ((steps + many_streams - 1) / many_streams * (rows > 128 ? 5000.0 : 7000.0) + 15000);
         if (many_cycles < few_cycles && many < (1ll << 27)) return launch_attention_prompt(a, cache.head_size, Half<T>::value, sequences, s);
     }
     CUtensorMap k_map, v_map;
