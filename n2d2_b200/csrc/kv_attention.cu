@@ -493,13 +493,13 @@ static cudaError_t launch_attention(const n2d2b_kv_cache& cache, const AttendArg
     // heads over 4000 38 / 70, 1 of 12 over 20000 50 / 92, 8 of 12 over 4000 44 / 66, 32 of 16 over 600 57 / 40, 32 of 32 over 1000 133 / 60, 8 of 64 of one
     // head over 64 15 / 9.
     const long long rows = (long long)a.c.max_new * a.group, key_heads = (long long)sequences * a.c.heads, steps = attend_steps(a);
-    if (rows > 16) {
+    if (rows > 16 || a.c.heads > 65535) {
         const long long few = (rows + 15) / 16 * key_heads, many = (rows + 255) / 256 * key_heads;
         const int few_streams = attend_streams(few, steps, 1, 8), many_streams = attend_streams(many, steps, 2, 8);
         const double sms = token_sms(), few_waves = few * few_streams / sms, many_waves = many * many_streams / sms;
         const double few_cycles = (few_waves > 1 ? few_waves : 1) * ((steps + few_streams - 1) / few_streams * 2000.0 + 12000);
         const double many_cycles = (many_waves > 1 ? many_waves : 1) * ((steps + many_streams - 1) / many_streams * (rows > 128 ? 5000.0 : 7000.0) + 15000);
-        if (many_cycles < few_cycles && many < (1ll << 27)) return launch_attention_prompt(a, cache.head_size, Half<T>::value, sequences, s);
+        if (many_cycles < few_cycles || (rows + 15) / 16 * a.c.heads > 65535) return launch_attention_prompt(a, cache.head_size, Half<T>::value, sequences, s);
     }
     CUtensorMap k_map, v_map;
     const unsigned long long lines = (unsigned long long)cache.nb_pages * cache.nb_heads * cache.page_tokens;
@@ -534,8 +534,9 @@ extern "C" int n2d2b_kv_attention(int device, const n2d2b_kv_cache* cache, const
         return set_error(N2D2B_ERR_INVALID, "strides must be 0 or multiples of 8 of at least %lld", (long long)width);
     if (!token_aligned(d.q, 16) || !token_aligned(d.out, 16)) return set_error(N2D2B_ERR_INVALID, "q and out must start on 16 bytes");
     a.group = d.nb_query_heads / cache->nb_heads;
-    if (((long long)a.c.max_new * a.group + 15) / 16 * cache->nb_heads > 65535)
-        return set_error(N2D2B_ERR_TOO_LARGE, "max_new x query heads exceeds %d rows", 65535 * 16);
+    const long long rows = (long long)a.c.max_new * a.group;
+    if (rows > (1 << 30) || (rows + 255) / 256 * cache->nb_heads * batch->nb_sequences >= (1ll << 27))
+        return set_error(N2D2B_ERR_TOO_LARGE, "max_new x query heads (x nb_sequences) exceeds what one call takes: 2^30 rows of a key head, 2^27 tiles of 256 of them");
     a.q = d.q; a.out = d.out;
     a.scale_log2 = d.scale * 1.4426950408889634f;
     a.causal = d.causal ? 1 : 0;

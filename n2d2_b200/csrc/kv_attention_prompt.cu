@@ -379,8 +379,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_attention_prompt_kernel(cons
                     }
                     const bool moves = best > top + 8.0f || (top == -INFINITY && best > top);       // (each row for itself: another row's numbers change nothing in it)
                     if (__any_sync(0xffffffffu, moves)) {
-                        const float fade = moves ? exp2_approx(top - best) : 1.0f;
-                        if (moves) top = best;
+                        // a whole number, so that the factor is a power of two and halves only lose what falls off their lower end
+                        const float raised = ceilf(best), fade = !moves ? 1.0f : (top == -INFINITY ? 0.0f : __int_as_float((127 + (int)fmaxf(top - raised, -127.0f)) << 23));
+                        if (moves) top = raised;
                         sum *= fade;
                         const __half2 fade2 = __float2half2_rn(fade);
 #pragma unroll 1

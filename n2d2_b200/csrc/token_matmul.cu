@@ -49,14 +49,15 @@ __device__ __forceinline__ void store_columns(const MatmulArgs& p, const unsigne
     }
 }
 
-// 16 bytes of k of a row that starts anywhere, zero from byte `valid` on: aligned words that hold a wanted byte, shifted into place
+// 16 bytes of k of a row that starts anywhere, zero from byte `valid` on: aligned words that hold a wanted byte (none of `valid` 0, wherever p
+// points), shifted into place
 __device__ __forceinline__ uint4 load_bytes(const int8_t* p, int valid)
 {
     const unsigned shift = (unsigned)((uintptr_t)p & 3u);
     const unsigned* const w = reinterpret_cast<const unsigned*>((uintptr_t)p - shift);
     unsigned x[5], r[4];
 #pragma unroll
-    for (int i = 0; i < 5; ++i) x[i] = 4 * i < (int)shift + valid ? w[i] : 0u;
+    for (int i = 0; i < 5; ++i) x[i] = valid > 0 && 4 * i < (int)shift + valid ? w[i] : 0u;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         r[i] = __funnelshift_r(x[i], x[i + 1], 8u * shift);
@@ -245,7 +246,10 @@ __device__ __forceinline__ void mbar_arrive_even(unsigned bar)
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(map_to_rank(bar, 0)) : "memory");
 }
 
-static constexpr int PAIR_STAGES = 6, PAIR_STAGE = 256 * MM_K, PAIR_SMEM = PAIR_STAGES * PAIR_STAGE + 1024, PAIR_THREADS = 320;
+static constexpr int PAIR_STAGES = 6, PAIR_STAGE = 256 * MM_K, PAIR_THREADS = 320;
+// all of TMEM, so all of the shared memory (see TMEM_BYTES)
+static constexpr int PAIR_SMEM = 227 * 1024 - 1024;
+static_assert(PAIR_STAGES * PAIR_STAGE + 1024 <= PAIR_SMEM, "the ring fits");
 
 // Persistent: a pair of blocks (one cta_group::2) walks over tiles of 256 channels x 256 tokens.  Each block holds its 128 channels and
 // half of the tokens of a step, so a byte is brought to a multiprocessor for twice the products of a single block's tile of 128 x 256; two

@@ -418,6 +418,33 @@ def test_attention_scales_of_any_size(news, size):
     check_attention(s, out)
 
 
+@pytest.mark.parametrize('order', ['rising', 'falling', 'jumping'])
+@pytest.mark.parametrize('size, page, new', [(128, 64, 1), (128, 16, 3), (64, 32, 1), (128, 64, 130), (128, 16, 70), (64, 16, 200)])
+def test_attention_maxima_that_move(size, page, new, order):
+    """Keys along the query, of scales that rise (or fall, or jump) from page to page: the maximum moves again and again, inside a step and between steps."""
+    s = Served([1500], [new], 1, size, page, 'bf16', heads=2)
+    used = s.table[0][:-(-1500 // page)]
+    s.k[used] = torch.where(s.q[0, 0] > 0, 1, -1).to(torch.int8) * torch.randint(1, 128, (len(used), 1, page, 1), device='cuda', generator=s.g).to(torch.int8)
+    rise = torch.linspace(0.01, 6.0, len(used), device='cuda')
+    if order == 'falling':
+        rise = rise.flip(0)
+    if order == 'jumping':
+        rise = rise[torch.randperm(len(used), device='cuda', generator=s.g)]
+    s.k_scales[used] = (rise / size ** 0.5)[:, None]
+    out = s.attention()
+    runtime.token_check()
+    check_attention(s, out)
+
+
+def test_attention_prompt_of_many_tiles():
+    """More rows than the other kernel's grid holds."""
+    s = Served([300], [300], 1, 64, 64, 'f16', heads=4)
+    s.batch.desc.max_new = 2 ** 19       # as a caller that knows no better bound
+    out = s.attention()
+    runtime.token_check()
+    check_attention(s, out)
+
+
 @pytest.mark.parametrize('power', [-120, -30, 30, 120])
 @pytest.mark.parametrize('new', [1, 40])
 def test_attention_queries_of_any_size(power, new):

@@ -96,7 +96,7 @@ def test_append_refuses(over, words, code):
     (dict(window=-1), 'window', INVALID), (dict(window=4, causal=0), 'window', INVALID), (dict(scale=float('nan')), 'scale', INVALID),
     (dict(scale=float('inf')), 'scale', INVALID), (dict(q=None), 'NULL', INVALID), (dict(out=BASE + 8), '16 bytes', INVALID),
     (dict(q_stride=255), 'strides', INVALID), (dict(out_stride=260), 'strides', INVALID),
-    (dict(max_new=2**20, nb_tokens=2**20, starts=BASE), 'exceeds', TOO_LARGE)])
+    (dict(max_new=2**30, nb_tokens=2**30, starts=BASE), 'exceeds', TOO_LARGE)])
 def test_attention_refuses(over, words, code):
     refused(attention(**over), words, code)
 
