@@ -347,13 +347,13 @@ int n2d2b_first_conv_noalloc_selftest_wait_timeout(int device, unsigned limit_us
  *   - take device buffers, on the given device (whichever is current; the caller's current device is left or put back), and
  *     enqueue their work on `stream`, without waiting, allocating or copying: they can be captured into a graph and replayed,
  *     and calls on several streams may overlap as long as none writes what another one reads or writes.  They use no
- *     workspace.  The first call of a kind on a device loads its kernel;
+ *     workspace.  The first call of a kind on a device loads its kernel: make it before a capture begins;
  *   - return N2D2B_ERR_INVALID for what they do not take, before any GPU work;
  *   - read and write rows of the given strides (in elements; 0: rows lie side by side) and nothing between or behind them;
  *   - make the same result from the same inputs, bit for bit, whatever ran beside them.
  * Buffers of one call may not overlap except where it says so.  A code q under a scale s stands for q * s, q in [-127, 127].
  * A scale comes of a largest magnitude a as a * (1 / 127); up to 2^-100 it is 0, and so are its codes.  A row or page that holds a
- * value that is not finite gets a scale that is not finite or not a number, and its values read as not a number.
+ * value that is not finite gets a scale that is not a number, and so do all of its values.
  */
 
 /* Waits for `stream` and returns N2D2B_ERR_TIMEOUT if a kernel of these operators gave up on a bounded wait on this device since the last

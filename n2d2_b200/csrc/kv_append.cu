@@ -33,7 +33,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvArgs c, const T*
 
     const int n = (hi - lo) * PER;
     uint4 kept[KEEP];
-    unsigned top = 0;
+    float most = 0.0f;
 #pragma unroll
     for (int i = 0; i < KEEP; ++i) {
         const int at = threadIdx.x + i * 256;
@@ -47,10 +47,10 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvArgs c, const T*
             float v[8];
             Elem<T>::unpack(kept[i], v);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) top = max(top, magnitude(v[e]));
+            for (int e = 0; e < 8; e += 2) most = largest(most, v[e], v[e + 1]);
         }
     }
-    top = __reduce_max_sync(0xffffffffu, top);
+    unsigned top = __reduce_max_sync(0xffffffffu, magnitude(most));
     if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
     __syncthreads();
 #pragma unroll
@@ -58,6 +58,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvArgs c, const T*
 
     float step = __uint_as_float(top) * TOKEN_STEP;
     if (step <= TOKEN_TINY) step = 0.0f;
+    if (top >= 0x7f800000u) step = __int_as_float(0x7fffffff);
     const float after = (before >= step || before != before) ? before : step;
     const float inverse = after > 0.0f ? 1.0f / after : 0.0f;
 #pragma unroll

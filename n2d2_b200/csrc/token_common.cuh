@@ -156,22 +156,23 @@ template <> struct Elem<__nv_bfloat16> {
     }
 };
 
-// Nearest whole number in [-127, 127]; what is no number becomes 0
-__device__ __forceinline__ int code_of(float v)
-{
-    int r;
-    asm("cvt.rni.s32.f32 %0, %1;" : "=r"(r) : "f"(fminf(fmaxf(v, -127.0f), 127.0f)));
-    return v != v ? 0 : r;
-}
+// Nearest whole number (ties to even) of a value within the codes' range, in the lowest byte: the sum with 1.5 * 2^23 rounds it there.  The product with the
+// reciprocal is rounded by itself first, as the codes' definition has it.  What is no number gets some code; its scale says what it is.
+__device__ __forceinline__ unsigned code_of(float v, float inverse) { return __float_as_uint(__fadd_rn(__fmul_rn(v, inverse), 12582912.0f)); }
 __device__ __forceinline__ unsigned pack_codes(const float* v, float inverse)
 {
-    unsigned w = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w |= ((unsigned)code_of(v[i] * inverse) & 0xffu) << (8 * i);
-    return w;
+    const unsigned ab = __byte_perm(code_of(v[0], inverse), code_of(v[1], inverse), 0x0040), cd = __byte_perm(code_of(v[2], inverse), code_of(v[3], inverse), 0x0040);
+    return __byte_perm(ab, cd, 0x5410);
 }
 
 // Magnitudes as whole numbers: their order is that of the values, with what is no number above everything, so a maximum keeps it
 __device__ __forceinline__ unsigned magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+// Largest magnitude, which stays no number once it is
+__device__ __forceinline__ float largest(float top, float a, float b)
+{
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(top), "f"(fabsf(a)), "f"(fabsf(b)));
+    return d;
+}
 
 }  // namespace n2d2b

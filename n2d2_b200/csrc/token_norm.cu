@@ -126,24 +126,25 @@ __global__ void __launch_bounds__(512) rmsnorm_quantize_kernel(const NormArgs a)
             }
         }
     };
-    auto weigh = [&](int i, float* v, float& sum, unsigned& top) {
+    auto weigh = [&](int i, float* v, float& sum, float& top) {
         float f[VEC];
         if (w) load(w + (size_t)i * VEC, f);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
             sum = fmaf(v[e], v[e], sum);
             if (w) v[e] *= f[e];
-            top = max(top, magnitude(v[e]));
         }
+#pragma unroll
+        for (int e = 0; e < VEC; e += 2) top = largest(top, v[e], v[VEC == 1 ? 0 : e + 1]);
     };
     auto store = [&](int i, const float* v, float inverse) {
-        if (VEC == 1) codes[i] = (int8_t)code_of(v[0] * inverse);
+        if (VEC == 1) codes[i] = (int8_t)code_of(v[0], inverse);
         else if (VEC == 4) *reinterpret_cast<unsigned*>(codes + (size_t)i * 4) = pack_codes(v, inverse);
         else *reinterpret_cast<uint2*>(codes + (size_t)i * 8) = make_uint2(pack_codes(v, inverse), pack_codes(v + 4, inverse));
     };
 
     float kept[(ITER ? ITER : 1) * VEC], sum = 0.0f;
-    unsigned top = 0;
+    float most = 0.0f;
     if (ITER) {
 #pragma unroll
         for (int k = 0; k < ITER; ++k) {
@@ -153,17 +154,19 @@ __global__ void __launch_bounds__(512) rmsnorm_quantize_kernel(const NormArgs a)
 #pragma unroll
         for (int k = 0; k < ITER; ++k) {
             const int i = threadIdx.x + k * blockDim.x;
-            if (i < n) weigh(i, kept + k * VEC, sum, top);
+            if (i < n) weigh(i, kept + k * VEC, sum, most);
         }
     } else {
         for (int i = threadIdx.x; i < n; i += blockDim.x) {
             sum_of(i, kept);
-            weigh(i, kept, sum, top);
+            weigh(i, kept, sum, most);
         }
     }
+    unsigned top = magnitude(most);
     block_sum_max(sum, top);
     float step = __uint_as_float(top) * TOKEN_STEP, inverse = 1.0f / step;
     if (step <= TOKEN_TINY) step = inverse = 0.0f;
+    if (top >= 0x7f800000u) step = __int_as_float(0x7fffffff);
     if (threadIdx.x == 0) a.scales[row] = step * rsqrtf(sum / (float)a.columns + a.eps);
     if (ITER) {
 #pragma unroll
@@ -176,7 +179,7 @@ __global__ void __launch_bounds__(512) rmsnorm_quantize_kernel(const NormArgs a)
         for (int i = threadIdx.x; i < n; i += blockDim.x) {
             float unused = 0.0f;
             load(h + (size_t)i * VEC, kept);
-            weigh(i, kept, unused, top);
+            weigh(i, kept, unused, most);
             store(i, kept, inverse);
         }
     }
