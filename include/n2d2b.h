@@ -353,7 +353,7 @@ int n2d2b_first_conv_noalloc_selftest_wait_timeout(int device, unsigned limit_us
  *   - make the same result from the same inputs, bit for bit, whatever ran beside them.
  * Buffers of one call may not overlap except where it says so.  A code q under a scale s stands for q * s, q in [-127, 127].
  * A scale comes of a largest magnitude a as a * (1 / 127); up to 2^-100 it is 0, and so are its codes.  A row or page that holds a
- * value that is not finite gets a scale that is not a number, and so do all of its values.
+ * value that is not finite gets a scale that is not a number, and every value of it reads as not a number.
  */
 
 /* Waits for `stream` and returns N2D2B_ERR_TIMEOUT if a kernel of these operators gave up on a bounded wait on this device since the last
