@@ -4,7 +4,7 @@
 //
 // The sums are exact in 32 bits, so any split of k gives the same bits.
 //
-// Few tokens are bound by bringing the weights (1 x 4096 x 4096: 6.5 us a call, 16.8 MB; 48 x 6144 x 4096: 9.2 us), many by the tensor pipe: 4096 x 4096 x 4096
+// Few tokens are bound by bringing the weights (1 x 4096 x 4096: 4.3 us, 16.8 MB; 48 x 6144 x 4096: 9.2 us), many by the tensor pipe: 4096 x 4096 x 4096
 // 47 to 57 us (2.9 to 2.4 POP/s with the clock that the power limit leaves; 79 % of the pipe's cycles).
 #include <cstdio>
 #include <cstring>
@@ -366,6 +366,52 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) matmul_i8_pair_kernel(const _
     }
 }
 
+// ---- a few tokens: no tiles
+// A warp takes two output channels, 512 bytes of k of both at a time, and M tokens: loads straight to registers, four products an instruction, one
+// sum over the warp at the end.  None of what a tile needs before its first and after its last byte (barriers, TMEM, a cluster's join).  1 x 4096 x
+// 4096: 4.3 us, 3.9 TB/s with launch and end; from three or four tokens on the products take longer than the bytes.
+template <typename T, int M, bool BYTES>
+__global__ void __launch_bounds__(256) matmul_i8_rows_kernel(const MatmulArgs p)
+{
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane = threadIdx.x & 31, n = ((int)blockIdx.x * 8 + (int)(threadIdx.x >> 5)) * 2;
+    if (n >= p.N) return;
+    const int8_t* const w0 = p.w + (size_t)n * p.w_stride;
+    const int8_t* const w1 = n + 1 < p.N ? w0 + p.w_stride : w0;
+    const int8_t* a[M];
+#pragma unroll
+    for (int m = 0; m < M; ++m) a[m] = p.a + (size_t)(m < p.M ? m : 0) * p.a_stride;
+    int acc[2][M] = {};
+    const auto load = [](const int8_t* from, int valid) { return BYTES ? load_bytes(from, valid) : *reinterpret_cast<const uint4*>(from); };
+#pragma unroll 4
+    for (int k = lane * 16; k < p.K; k += 512) {
+        const int valid = min(p.K - k, 16);
+        const uint4 x0 = load(w0 + k, valid), x1 = load(w1 + k, valid);
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+            const uint4 y = load(a[m] + k, valid);
+            acc[0][m] = __dp4a((int)x0.w, (int)y.w, __dp4a((int)x0.z, (int)y.z, __dp4a((int)x0.y, (int)y.y, __dp4a((int)x0.x, (int)y.x, acc[0][m]))));
+            acc[1][m] = __dp4a((int)x1.w, (int)y.w, __dp4a((int)x1.z, (int)y.z, __dp4a((int)x1.y, (int)y.y, __dp4a((int)x1.x, (int)y.x, acc[1][m]))));
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int sum = __reduce_add_sync(0xffffffffu, acc[r][m]);
+            if (lane == 2 * m + r && m < p.M && n + r < p.N)
+                ((T*)p.out)[(size_t)m * p.out_stride + n + r] = Elem<T>::from_float(fmaf((float)sum * p.a_scales[m], p.w_scales[n + r], p.bias ? p.bias[n + r] : 0.0f));
+        }
+}
+
+template <typename T, int M>
+static cudaError_t launch_few(const MatmulArgs& p, bool bytes, cudaStream_t s)
+{
+    const dim3 grid((unsigned)((p.N + 15) / 16));
+    return bytes ? launch_token(matmul_i8_rows_kernel<T, M, true>, grid, 256, 0, 1, s, p) : launch_token(matmul_i8_rows_kernel<T, M, false>, grid, 256, 0, 1, s, p);
+}
+
 // Blocks that share a multiprocessor so that all of a call run at once, four at most (their rings get the smaller for it)
 static int tile_residents(const MatmulArgs& p, int sms, int bn, int split)
 {
@@ -445,6 +491,15 @@ template <typename T>
 static cudaError_t launch_matmul(const MatmulArgs& p, cudaStream_t s)
 {
     const bool bytes = !token_aligned(p.a, 16) || !token_aligned(p.w, 16) || p.a_stride % 16 || p.w_stride % 16;
+    // one or two tokens, up to eight where the products are few or the rows would have to come through registers anyway (us, tiles / without: 1 x 4096 x 4096
+    // 6.6 / 4.3, 2 x 4096 x 4096 6.6 / 4.5, 4 x 1024 x 4096 5.4 / 4.7, 8 x 4096 x 4096 6.7 / 7.0, 4 x 8192 x 4096 8.8 / 13.8; unaligned 2 x 1024 x 1199 12.1 / 4.2, 8 x
+    // 1024 x 1199 12.2 / 10.8)
+    if (p.M <= 2 || (p.M <= 8 && (bytes || (long long)p.M * p.N * p.K <= 1 << 25))) {
+        const bool words = bytes || p.K % 16;
+        if (p.M == 1) return launch_few<T, 1>(p, words, s);
+        if (p.M == 2) return launch_few<T, 2>(p, words, s);
+        return p.M <= 4 ? launch_few<T, 4>(p, words, s) : launch_few<T, 8>(p, words, s);
+    }
     int* const status = token_status_word();
     if (!status) return cudaErrorInvalidSymbol;
     const int sms = token_sms(), blocks = (p.K + MM_K - 1) / MM_K;
