@@ -72,9 +72,11 @@ __device__ __forceinline__ uint4 load_bytes(const int8_t* p, int valid)
 
 // One tile of 128 channels x BN tokens a block.  Few tiles: the blocks of a cluster take parts of k and add their 32-bit sums up through
 // distributed shared memory, each finishing a share of the tile.  Warp 0 loads, warp 1 issues the MMAs, four warps store.  BYTES: rows that TMA cannot read (not on 16
-// bytes); the storing warps bring them through registers first.
+// bytes); twelve warps, the storing ones among them, bring them through registers first: 64 bytes a thread are under way at a time (with four warps
+// 1156 x 1024 x 3277 took 112 us, with twelve 47).
+template <bool BYTES> struct TileWarps { static constexpr int BRINGING = BYTES ? 12 : 4, THREADS = 64 + 32 * BRINGING; };
 template <typename T, int BN, bool BYTES>
-__global__ void __launch_bounds__(192, 1) matmul_i8_tile_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap a_map, const MatmulArgs p,
+__global__ void __launch_bounds__(TileWarps<BYTES>::THREADS, 1) matmul_i8_tile_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap a_map, const MatmulArgs p,
                                                                 int stages, int* status)
 {
     constexpr int STAGE = (128 + BN) * MM_K, COLUMNS = BN < 32 ? 32 : BN;
@@ -86,7 +88,7 @@ __global__ void __launch_bounds__(192, 1) matmul_i8_tile_kernel(const __grid_con
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         if (!BYTES) { prefetch_tensor_map(&w_map); prefetch_tensor_map(&a_map); }
-        for (int i = 0; i < stages; ++i) { mbar_init(smem_u32(&full[i]), BYTES ? 4 : 1); mbar_init(smem_u32(&empty[i]), 1); }
+        for (int i = 0; i < stages; ++i) { mbar_init(smem_u32(&full[i]), BYTES ? TileWarps<BYTES>::BRINGING : 1); mbar_init(smem_u32(&empty[i]), 1); }
         mbar_init(smem_u32(&done), 1);
         abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -138,26 +140,27 @@ __global__ void __launch_bounds__(192, 1) matmul_i8_tile_kernel(const __grid_con
             __syncwarp();
         }
     } else {
-        for (int i = (int)threadIdx.x - 64; i < BN; i += 128) sa[i] = t0 + i < p.M ? p.a_scales[t0 + i] : 0.0f;
+        constexpr int BRINGING = 32 * TileWarps<BYTES>::BRINGING;
+        for (int i = (int)threadIdx.x - 64; i < BN; i += BRINGING) sa[i] = t0 + i < p.M ? p.a_scales[t0 + i] : 0.0f;
         const int tid = (int)threadIdx.x - 64, chunk = tid & 7;
         for (int i = 0; BYTES && i < count; ++i) {
             const int slot = i % stages, k = (from + i) * MM_K + chunk * 16, valid = min(max(p.K - k, 0), 16);
             if (i >= stages && !mbar_wait_warp(smem_u32(&empty[slot]), (unsigned)(i / stages - 1) & 1u, &abort_flag, status, 31)) break;
             const unsigned dst = smem_u32(smem) + (unsigned)(slot * STAGE);
-            // rows tid / 8, + 16, ...: four at a time, so that their loads are under way together
+            // rows tid / 8, + BRINGING / 8, ...: four at a time, so that their loads are under way together
 #pragma unroll 1
-            for (int r0 = tid >> 3; r0 < 128 + BN; r0 += 64) {
+            for (int r0 = tid >> 3; r0 < 128 + BN; r0 += BRINGING / 2) {
                 uint4 v[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int r = r0 + 16 * e, row = r < 128 ? n0 + r : t0 + r - 128;
+                    const int r = r0 + BRINGING / 8 * e, row = r < 128 ? n0 + r : t0 + r - 128;
                     const bool there = r < 128 + BN && row < (r < 128 ? p.N : p.M);
                     const int8_t* const at = r < 128 ? p.w + (size_t)row * p.w_stride + k : p.a + (size_t)row * p.a_stride + k;
                     v[e] = load_bytes(at, there ? valid : 0);
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int r = r0 + 16 * e;
+                    const int r = r0 + BRINGING / 8 * e;
                     if (r < 128 + BN)
                         asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst + (unsigned)(r * MM_K + ((chunk ^ (r & 7)) << 4))), "r"(v[e].x), "r"(v[e].y),
                                      "r"(v[e].z), "r"(v[e].w) : "memory");
@@ -174,7 +177,7 @@ __global__ void __launch_bounds__(192, 1) matmul_i8_tile_kernel(const __grid_con
     if (!ok) __nanosleep(1000000);      // copies under way land before the block leaves
     // the ring is free: every MMA has read its operands
     int* const part = (int*)smem;       // [token][128 channels]
-    if (warp >= 2) {
+    if (warp >= 2 && warp < 6) {
         const int quad = warp & 3, channel = quad * 32 + lane;
         const float sw = ranks == 1 && n0 + channel < p.N ? p.w_scales[n0 + channel] : 0.0f;
         const float bias = ranks == 1 && p.bias && n0 + channel < p.N ? p.bias[n0 + channel] : 0.0f;
@@ -439,7 +442,7 @@ static cudaError_t launch_tile(const MatmulArgs& p, int split, int* status, cuda
     const cudaError_t e = raise_smem_limit(matmul_i8_tile_kernel<T, BN, BYTES>, set, TILE_RING + 1024);
     if (e != cudaSuccess) return e;
     const dim3 grid((unsigned)split, (unsigned)((p.N + 127) / 128), (unsigned)((p.M + BN - 1) / BN));
-    return launch_token(matmul_i8_tile_kernel<T, BN, BYTES>, grid, 192, bytes, split, s, w_map, a_map, p, stages, status);
+    return launch_token(matmul_i8_tile_kernel<T, BN, BYTES>, grid, TileWarps<BYTES>::THREADS, bytes, split, s, w_map, a_map, p, stages, status);
 }
 
 template <typename T>
@@ -470,8 +473,8 @@ static double expected_cycles(const MatmulArgs& p, int sms, int bn, int split, b
     const long long ctas = (long long)((p.N + 127) / 128) * ((p.M + bn - 1) / bn) * split, each = (ctas + sms - 1) / sms;
     if (split == 8 && each > 1) return 1e30;       // (clusters of eight find no place beside one another: 14.4 us instead of 9.7 for 48 x 6144 x 4096)
     const long long residents = tile_residents(p, sms, bn, split), rounds = (each + residents - 1) / residents;
-    // a step's MMAs (128 cycles for 256 tokens, no fewer than 50 an MMA), or its bytes at 45 a cycle (through registers: 12)
-    const double mma = bn >= 128 ? bn * 2 : 200, load = (128 + bn) * MM_K / (bytes ? 12.0 : 45.0), share = ctas > sms ? (double)ctas / sms : 1.0;
+    // a step's MMAs (128 cycles for 256 tokens, no fewer than 50 an MMA), or its bytes at 45 a cycle (through registers: 5.7, and a block's rate does not rise where others leave early)
+    const double mma = bn >= 128 ? bn * 2 : 200, load = (128 + bn) * MM_K / (bytes ? 5.7 : 45.0), share = bytes ? (double)each : ctas > sms ? (double)ctas / sms : 1.0;
     return 3000 + share * (((p.K + MM_K - 1) / MM_K + split - 1) / split) * (mma > load ? mma : load) + rounds * (1050 + bn * 9.0) + (split > 1 ? 2700 + bn * (26 + 0.4 * split) : 0.0);
 }
 
