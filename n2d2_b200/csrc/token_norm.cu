@@ -239,6 +239,9 @@ extern "C" int n2d2b_rmsnorm_quantize(int device, const n2d2b_norm* norm, n2d2b_
     a.codes_stride = d.codes_stride ? d.codes_stride : d.columns;
     if (a.x_stride < d.columns || a.residual_stride < d.columns || a.total_stride < d.columns || a.codes_stride < d.columns)
         return set_error(N2D2B_ERR_INVALID, "strides must be 0 or at least the %d columns of a row", d.columns);
+    // (rows that another row's sum overwrites before they are read)
+    if (d.total && ((d.total == d.x && a.total_stride != a.x_stride) || (d.total == d.residual && a.total_stride != a.residual_stride)))
+        return set_error(N2D2B_ERR_INVALID, "total in the place of x or residual takes the same stride");
     const TokenDevice on(device);
     if (on.err != cudaSuccess) return set_error(N2D2B_ERR_CUDA, "device %d is not usable: %s", device, cudaGetErrorString(on.err));
     cudaError_t e;

@@ -66,6 +66,17 @@ def test_norm_refuses(over, words):
     refused(norm(**over), words)
 
 
+@pytest.mark.parametrize('over, refuses', [
+    (dict(x_stride=128, residual=BASE + 1024, total=BASE), True), (dict(residual=BASE + 1024, residual_stride=128, total=BASE + 1024), True),
+    (dict(residual=BASE + 1024, total=BASE, total_stride=128), True), (dict(x_stride=128, residual=BASE + 1024, total=BASE, total_stride=128), False),
+    (dict(x_stride=64, residual=BASE + 1024, total=BASE), False), (dict(x_stride=128, residual=BASE + 1024, total=BASE + 1024), False)])
+def test_norm_refuses_a_sum_that_overwrites_other_rows(over, refuses):
+    if refuses:
+        refused(norm(**over), 'same stride')
+    else:       # nothing to say about the strides: the next refusal answers
+        refused(norm(codes_stride=8, **over), 'columns of a row')
+
+
 @pytest.mark.parametrize('over, words, code', [
     (dict(dtype=1), 'dtype', INVALID), (dict(m=-1), 'size', INVALID), (dict(n=0), 'size', INVALID), (dict(k=0), 'size', INVALID),
     (dict(k=131072), '131071', TOO_LARGE), (dict(m=65535 * 64 + 1), 'exceeds', TOO_LARGE), (dict(n=65535 * 128 + 1, out_stride=2**24), 'exceeds', TOO_LARGE), (dict(a=None), 'NULL', INVALID),
