@@ -494,10 +494,10 @@ template <typename T>
 static cudaError_t launch_matmul(const MatmulArgs& p, cudaStream_t s)
 {
     const bool bytes = !token_aligned(p.a, 16) || !token_aligned(p.w, 16) || p.a_stride % 16 || p.w_stride % 16;
-    // one or two tokens, up to eight where the products are few or the rows would have to come through registers anyway (us, tiles / without: 1 x 4096 x 4096
-    // 6.6 / 4.3, 2 x 4096 x 4096 6.6 / 4.5, 4 x 1024 x 4096 5.4 / 4.7, 8 x 4096 x 4096 6.7 / 7.0, 4 x 8192 x 4096 8.8 / 13.8; unaligned 2 x 1024 x 1199 12.1 / 4.2, 8 x
-    // 1024 x 1199 12.2 / 10.8)
-    if (p.M <= 2 || (p.M <= 8 && (bytes || (long long)p.M * p.N * p.K <= 1 << 25))) {
+    // one or two tokens, up to eight where the products are few (us, tiles / without: 1 x 4096 x 4096 6.6 / 4.3, 2 x 4096 x 4096 6.6 / 4.5, 4 x 1024 x 4096
+    // 5.4 / 4.7, 8 x 4096 x 4096 6.7 / 7.0, 4 x 8192 x 4096 8.8 / 13.8).  Unaligned rows: one token, up to four short ones (1 x 4096 x 5999 23.8 / 17.2, 4 x
+    // 10000 x 511 10.5 / 6.9, 4 x 1000 x 999 6.1 / 5.3, 2 x 4096 x 2001 9.3 / 10.8, 4 x 4096 x 4001 14.5 / 24.5, 6 x 1000 x 999 6.1 / 8.1)
+    if (bytes ? p.M == 1 || (p.M <= 4 && p.M * p.K <= 4000) : p.M <= 2 || (p.M <= 8 && (long long)p.M * p.N * p.K <= 1 << 25)) {
         const bool words = bytes || p.K % 16;
         if (p.M == 1) return launch_few<T, 1>(p, words, s);
         if (p.M == 2) return launch_few<T, 2>(p, words, s);
