@@ -3,7 +3,7 @@
 //   s_j = scale * sK(page of j) * (q . k_j),   out = (sum_j e^(s_j) sV(page of j) v_j) / (sum_j e^(s_j))      over visible j
 //
 // in one pass over the tokens, with the running maximum of t_j = s_j log2(e) + log2 sV(page of j): the values' scales ride in the
-// exponent, so that p_j = 2^(t_j - max) is at most 1 whatever the scales are and enters the second product in 16 bits; the softmax's sum
+// exponent, so that p_j = 2^(t_j - max) is at most 1 whatever the scales are and enters the second product in few bits; the softmax's sum
 // adds p_j / sV(page of j).
 //
 // kv_attention_rows_kernel: 8 or 16 rows (new token x query head of one key head) a tile, for few rows: bound by reading the cache.  The

@@ -7,7 +7,8 @@
 //   warps 12-19  a thread holds one row of one tile: scores to probabilities, running maximum and sum, at the end O / sum
 // While the tensor pipe works on one tile, the other tile's rows are in the hands of their threads, 32 scores at a time with the next 32 on
 // their way.  A row's maximum only moves, and the output so far is only rescaled, when a score is more than 2^8 above it: below that the
-// probabilities stay far inside 16 bits and their sum in 32 whatever the maximum they are taken against.
+// probabilities stay inside 16 bits and their sum in 32 whatever the maximum they are taken against.  A probability of 1 is 2^5 to 2^6 there, so one
+// keeps its 11 bits down to 2^-19 and is off by at most 2^-30 below that.
 //
 // 4096 new tokens over 8192 (32 query heads, 8 key heads of 128, bf16): 509 to 520 us, 790 to 810 TFLOP/s, 48 % of what a large matrix product reaches.  Bound by
 // the latency of a row's chain (scores out of TMEM, maximum, exponentials, back into TMEM) with two warps of rows to a scheduler: no pipe is more than
@@ -20,6 +21,7 @@
 namespace n2d2b {
 
 static constexpr int PR_THREADS = 640, PR_BLOCK = 128, PR_CONSTS = 4, PR_POLYNOMIAL = 6;
+static constexpr float PR_BITS = 6.0f, PR_ROOM = 8.0f;       // a probability of 1 is 2^5 to 2^6, the largest before the maximum moves 2^14
 template <int D> struct PromptSmem {
     static constexpr int TILE = 128 * D * 2;                 // 128 rows (or tokens) of halves, in blocks of 64 columns
     static constexpr int Q = 0, K = Q + 2 * TILE, V = K + 2 * TILE, NEED = V + 2 * TILE + 1024;
@@ -99,7 +101,7 @@ __device__ __forceinline__ float max_of(float a, float b, float c)
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-// 2^x for x up to 8 without the exponential unit, which a quarter of the probabilities is kept from (it takes 8 cycles for a warp's 32 and would bound
+// 2^x for x up to 14 without the exponential unit, which a quarter of the probabilities is kept from (it takes 8 cycles for a warp's 32 and would bound
 // the kernel): x = n + f with n whole, 2^f on [-1/2, 1/2] by the polynomial of degree 4 with the smallest relative error (2.6e-6, from an exchange
 // iteration), n added to its exponent.  Below 2^-126 the result is that.
 __device__ __forceinline__ Pair exp2_pair(Pair x)
@@ -382,10 +384,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_attention_prompt_kernel(cons
                         const float most = max_of(max_of(m[0], m[1], m[2]), max_of(m[3], m[4], __uint_as_float(x[16 * g + 15])), -INFINITY);
                         best = fmaxf(best, MASKED && most == -INFINITY ? -INFINITY : fmaf(most, f[g].x * row_scale, f[g].y));
                     }
-                    const bool moves = best > top + 8.0f || (top == -INFINITY && best > top);       // (each row for itself: another row's numbers change nothing in it)
+                    const bool moves = best > top + (PR_BITS + PR_ROOM) || (top == -INFINITY && best > top);       // (each row for itself: another row's numbers change nothing in it)
                     if (__any_sync(0xffffffffu, moves)) {
                         // a whole number, so that the factor is a power of two and halves only lose what falls off their lower end
-                        const float raised = ceilf(best), fade = !moves ? 1.0f : (top == -INFINITY ? 0.0f : __int_as_float((127 + (int)fmaxf(top - raised, -127.0f)) << 23));
+                        const float raised = ceilf(best) - PR_BITS, fade = !moves ? 1.0f : (top == -INFINITY ? 0.0f : __int_as_float((127 + (int)fmaxf(top - raised, -127.0f)) << 23));
                         if (moves) top = raised;
                         sum *= fade;
                         const __half2 fade2 = __float2half2_rn(fade);

@@ -445,6 +445,30 @@ def test_attention_prompt_of_many_tiles():
     check_attention(s, out)
 
 
+@pytest.mark.parametrize('kv_heads, new', [(8, 300), (1, 1)])
+def test_attention_small_probabilities_beside_a_large_one_of_nothing(kv_heads, new):
+    """What is left when the token that nearly has it all holds zeros: probabilities of e^-10 to e^-16."""
+    s = Served([3], [new], kv_heads, 64, 16, 'f16', heads=4 * kv_heads)
+    page, signs = s.table[0][0], torch.where(torch.arange(64, device='cuda') % 3 == 0, -1.0, 1.0)
+    s.k_scales.fill_(1 / 127)
+    s.k[page, :, 0] = (127 * signs).to(torch.int8)
+    s.v_scales.fill_(5.0)
+    s.v[page, :, 0] = 0
+    s.q.copy_((1 + 0.5 * torch.rand(s.q.shape[:2] + (1,), device='cuda', generator=s.g)) * signs)
+    out = s.attention(scale=1 / 6, causal=False)
+    runtime.token_check()
+    check_attention(s, out, causal=False, scale=1 / 6)
+
+
+@pytest.mark.parametrize('new', [1, 40])
+@pytest.mark.parametrize('size', [64, 128])
+def test_attention_of_a_negative_scale(new, size):
+    s = Served([300, 41], [new, new], 2, size, 32, 'bf16', heads=8)
+    out = s.attention(scale=-0.1)
+    s.q.neg_()
+    check_attention(s, out, scale=0.1)
+
+
 @pytest.mark.parametrize('power', [-120, -30, 30, 120])
 @pytest.mark.parametrize('new', [1, 40])
 def test_attention_queries_of_any_size(power, new):
