@@ -16,7 +16,7 @@
 // up to 16 blocks, whose parts are joined through distributed shared memory at the end: nothing is kept in memory between kernels.
 //
 // 48 sequences of up to 8000 tokens (8 key heads of 128, 32 query heads, bf16): 81 to 85 us, 5.7 to 6.0 TB/s; one of 65000: 33 us, 4.0 TB/s (128 of the
-// multiprocessors, a cluster of 16 for each head; the blocks' beginning and end take a third of it); 100 tokens, heads of 64: 5.7 us a call.
+// multiprocessors, a cluster of 16 for each head; the blocks' beginning and end take 8 us of it); 100 tokens, heads of 64: 5.7 us a call.
 #include <cstdio>
 #include <cstring>
 #include "kv_common.cuh"
