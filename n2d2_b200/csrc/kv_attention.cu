@@ -4,7 +4,7 @@
 //
 // in one pass over the tokens, with the running maximum of t_j = s_j log2(e) + log2 sV(page of j): the values' scales ride in the
 // exponent, so that p_j = 2^(t_j - max) is at most 1 whatever the scales are and enters the second product in few bits; the softmax's sum
-// adds p_j / sV(page of j).
+// adds p_j / sV(page of j): the p_j of that sum are about 1, as the scales go from 2^-100 to 2^121 and their reciprocals fill 32 bits.
 //
 // kv_attention_rows_kernel: 8 or 16 rows (new token x query head of one key head) a tile, for few rows: bound by reading the cache.  The
 // codes go into the int8 tensor cores as they lie in memory: widening them in registers took 224 integer instructions a warp for 32
@@ -62,7 +62,8 @@ __device__ __forceinline__ float float_of(unsigned x, float by) { return fmaf(__
 
 static constexpr int ROWS_BLOCK = 128, ROWS_GROUP = 192;
 static constexpr int ROWS_FLUSH = 512;          // blocks whose sums stay within 32 bits: 512 x 128 x 255 x 128 < 2^31
-static constexpr float ROWS_BITS = 23.0f;       // a probability of 1 is 2^23: 2^8 times as much still fits 32 bits
+static constexpr float ROWS_ONE = 0x1p23f;      // the whole number of a probability of 1: 2^8 times as much still fits 32 bits
+static constexpr float ROWS_ROOM = 8.0f;        // powers of two that a score may be above the maximum before that moves
 static constexpr float ROWS_NONE = -3.0e38f;    // the maximum of nothing
 // R: rows of a tile (4, 8 or 16); GROUPS: streams of tokens in a block
 template <int D, int R, int GROUPS> struct RowsSmem {
@@ -259,7 +260,7 @@ __global__ void __launch_bounds__(ROWS_GROUP * GROUPS, GROUPS == 2 ? 1 : R == 16
             for (int i = place; i < 2 * S::NP * ROWS_BLOCK / 16; i += 128) *reinterpret_cast<uint4*>(p_smem + 16 * i) = make_uint4(0, 0, 0, 0);
         bool ok = mbar_wait_warp(smem_u32(&q_full), 0, &abort_flag, a.status, 29);
 
-        // base: a row's maximum so far less the bits of a probability of 1
+        // from: the maximum that a row's probabilities are taken against
         float row_scale[R], from[R], sum[R], acc[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -281,7 +282,7 @@ __global__ void __launch_bounds__(ROWS_GROUP * GROUPS, GROUPS == 2 ? 1 : R == 16
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 const float high = fmaf((float)(int)x[4 * r + 3], 256.0f, (float)(int)x[4 * r + 2]), low = fmaf((float)(int)x[4 * r + 1], 256.0f, (float)(int)x[4 * r]);
-                acc[r] += fmaf(high, 65536.0f, low);
+                acc[r] = fmaf(fmaf(high, 65536.0f, low), 1.0f / ROWS_ONE, acc[r]);
             }
             pending = 0;
         };
@@ -305,7 +306,7 @@ __global__ void __launch_bounds__(ROWS_GROUP * GROUPS, GROUPS == 2 ? 1 : R == 16
 #pragma unroll 1
         for (int j = 0; j < blocks; ++j) {
             const int token = token0 + j * ROWS_BLOCK, j0 = token - place;
-            const float k_scale = bad_next ? __int_as_float(0x7fffffff) : k_next, v_scale = v_next <= TOKEN_TINY ? TOKEN_TINY : v_next;   // (all codes are 0 there)
+            const float k_scale = bad_next ? __int_as_float(0x7fffffff) : k_next, v_scale = v_next <= TOKEN_TINY ? KV_NOTHING : v_next;   // (all codes are 0 there)
             if (j + 1 < blocks) scales_of(number_next);
             number_next = number_of(j + 2);
             const float v_log = __log2f(v_scale), v_inverse = exp2_approx(-v_log);
@@ -329,8 +330,8 @@ __global__ void __launch_bounds__(ROWS_GROUP * GROUPS, GROUPS == 2 ? 1 : R == 16
             }
 #pragma unroll
             for (int r = 0; r < R; ++r) over = fmaxf(over, t[r] - from[r]);
-            // the maximum only moves when a score is more than 2^8 above it: below that, nothing leaves the digits
-            const bool move = any_of_128(group, over > ROWS_BITS + 8.0f);
+            // below that room nothing leaves the digits
+            const bool move = any_of_128(group, over > ROWS_ROOM);
             if (move) {
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
@@ -348,7 +349,7 @@ __global__ void __launch_bounds__(ROWS_GROUP * GROUPS, GROUPS == 2 ? 1 : R == 16
             if (move) {
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
-                    const float m = fmaxf(fmaxf(fmaxf(tops[group][0][r], tops[group][1][r]), fmaxf(tops[group][2][r], tops[group][3][r])) - ROWS_BITS, from[r]);
+                    const float m = fmaxf(fmaxf(fmaxf(tops[group][0][r], tops[group][1][r]), fmaxf(tops[group][2][r], tops[group][3][r])), from[r]);
                     const float fade = exp2_approx(from[r] - m);
                     from[r] = m;
                     sum[r] *= fade;
@@ -360,7 +361,7 @@ __global__ void __launch_bounds__(ROWS_GROUP * GROUPS, GROUPS == 2 ? 1 : R == 16
             for (int r = 0; r < R; ++r) {
                 const float p = exp2_approx(t[r] - from[r]);
                 if (whole || p != 0.0f) sum[r] = fmaf(p, v_inverse, sum[r]);     // (the scale of a page that a row does not see may be anything)
-                digits[r] = __float2uint_rn(p);                                  // its bytes are the digits, the lowest first
+                digits[r] = __float2uint_rn(p * ROWS_ONE);                       // its bytes are the digits, the lowest first
             }
             // the place is free when the products of the block before the last are through
             if (j >= 2) ok = ok && mbar_wait_warp(smem_u32(&bars.o_done[slot2]), phase2, &abort_flag, a.status, 28);

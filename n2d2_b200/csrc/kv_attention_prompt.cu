@@ -8,7 +8,8 @@
 // While the tensor pipe works on one tile, the other tile's rows are in the hands of their threads, 32 scores at a time with the next 32 on
 // their way.  A row's maximum only moves, and the output so far is only rescaled, when a score is more than 2^8 above it: below that the
 // probabilities stay inside 16 bits and their sum in 32 whatever the maximum they are taken against.  A probability of 1 is 2^5 to 2^6 there, so one
-// keeps its 11 bits down to 2^-19 and is off by at most 2^-30 below that.
+// keeps its 11 bits down to 2^-19 and is off by at most 2^-30 below that.  The softmax's sum is held on 2^-4 of that scale: it adds reciprocals of the values' scales
+// from 2^-121 to 2^100.
 //
 // 4096 new tokens over 8192 (32 query heads, 8 key heads of 128, bf16): 509 to 520 us, 790 to 810 TFLOP/s, 48 % of what a large matrix product reaches.  Bound by
 // the latency of a row's chain (scores out of TMEM, maximum, exponentials, back into TMEM) with two warps of rows to a scheduler: no pipe is more than
@@ -21,6 +22,7 @@
 namespace n2d2b {
 
 static constexpr int PR_THREADS = 640, PR_BLOCK = 128, PR_CONSTS = 4, PR_POLYNOMIAL = 6;
+static constexpr float PR_SUM = 4.0f;                        // powers of two that the sum's probabilities are below those of the products (0x1p-4f at the end)
 static constexpr float PR_BITS = 6.0f, PR_ROOM = 8.0f;       // a probability of 1 is 2^5 to 2^6, the largest before the maximum moves 2^14
 template <int D> struct PromptSmem {
     static constexpr int TILE = 128 * D * 2;                 // 128 rows (or tokens) of halves, in blocks of 64 columns
@@ -130,7 +132,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_attention_prompt_kernel(cons
     typedef PromptSmem<D> S;
     unsigned char* const smem = (unsigned char*)(((uintptr_t)dyn_smem() + 1023) & ~(uintptr_t)1023);
     __shared__ __align__(8) PromptBars bars;
-    __shared__ float4 consts[PR_CONSTS][PR_BLOCK / 16];     // scale of the keys, log2 and reciprocal of the values', for 16 tokens
+    __shared__ float4 consts[PR_CONSTS][PR_BLOCK / 16];     // scale of the keys, log2 and reciprocal (times 2^-PR_SUM) of the values', for 16 tokens
     __shared__ float part_top[256], part_sum[256];
     __shared__ unsigned tmem_slot;
     __shared__ int abort_flag;
@@ -203,8 +205,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_attention_prompt_kernel(cons
             for (int j = 0; j < blocks; ++j) {
                 if (j >= PR_CONSTS && !mbar_wait_issuer(smem_u32(&bars.c_empty[j & (PR_CONSTS - 1)]), (unsigned)(j / PR_CONSTS - 1) & 1u, &abort_flag, a.status, 46)) break;
                 if (lane < 8) {
-                    const float scale = v_scale <= TOKEN_TINY ? TOKEN_TINY : v_scale, log = __log2f(scale);       // (all codes are 0 there)
-                    consts[j & (PR_CONSTS - 1)][lane] = make_float4(bad ? __int_as_float(0x7fffffff) : k_scale, log, exp2_approx(-log), 0.0f);
+                    const float scale = v_scale <= TOKEN_TINY ? KV_NOTHING : v_scale, log = __log2f(scale);       // (all codes are 0 there)
+                    consts[j & (PR_CONSTS - 1)][lane] = make_float4(bad ? __int_as_float(0x7fffffff) : k_scale, log, exp2_approx(-log - PR_SUM), 0.0f);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&bars.c_full[j & (PR_CONSTS - 1)]));
@@ -498,7 +500,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_attention_prompt_kernel(cons
                 part_sum[i * 128 + r] = sum;
             } else {
             tc_fence_after();
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const float inv = sum == 0.0f ? 0.0f : 0x1p-4f / sum;
             T* const out = (T*)a.out + (size_t)(s.first_row + t) * a.out_stride + (size_t)(head * a.group + h) * D;
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
@@ -538,7 +540,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_attention_prompt_kernel(cons
                 o.x = fmaf(x.x, f, o.x); o.y = fmaf(x.y, f, o.y); o.z = fmaf(x.z, f, o.z); o.w = fmaf(x.w, f, o.w);
                 l = fmaf(ld_cluster(map_to_rank(at_sum, k)), f, l);
             }
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            const float inv = l == 0.0f ? 0.0f : 0x1p-4f / l;
             const int row = row0 + r, t = row / a.group, h = row - t * a.group;
             T* const out = (T*)a.out + (size_t)(s.first_row + t) * a.out_stride + (size_t)(head * a.group + h) * D + d;
             *reinterpret_cast<uint2*>(out) = make_uint2(Elem<T>::pack2(o.x * inv, o.y * inv), Elem<T>::pack2(o.z * inv, o.w * inv));

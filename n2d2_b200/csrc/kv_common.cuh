@@ -76,6 +76,10 @@ struct AttendArgs {
     int* status;
 };
 
+// What stands for a scale of zero (up to TOKEN_TINY) of a page's values in the exponents: any number would do, as its codes are zeros.  This one is below the scales that a
+// page of ordinary values has beside it, so its probabilities take no bits from theirs, and its reciprocal leaves the softmax's sum in 32 bits room for 2^40 tokens.
+static constexpr float KV_NOTHING = 8.271806125530277e-25f;    // 2^-80
+
 // (bytes 0, 1) and (bytes 2, 3) of four codes + 128 as halves 1024 + u
 __device__ __forceinline__ unsigned splice(unsigned w, unsigned sel)
 {

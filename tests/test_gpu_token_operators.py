@@ -656,3 +656,62 @@ def test_long_cache_offsets_leave_32_bits():
     runtime.token_check()
     assert not k[:1000].any() and bool(k[last].any())
     check_attention(s, out)
+
+
+def nothing(s, b, places):
+    """Values of zero at places [lo, hi) of sequence b, as append leaves them: where a whole page has none its scale is 0."""
+    for lo, hi in places:
+        for t in range(lo, hi, s.page):
+            assert lo % s.page == 0
+            n = min(s.page, hi - t)
+            s.v[s.table[b][t // s.page], :, :n] = 0
+            if n == s.page or t + n >= s.lengths[b]:
+                s.v_scales[s.table[b][t // s.page]] = 0
+
+
+@pytest.mark.parametrize('new', [1, 3, 40, 300])
+@pytest.mark.parametrize('size, page, length, places', [
+    (128, 64, 256, [(0, 128)]), (64, 16, 512, [(0, 256)]), (128, 64, 512, [(256, 512)]), (64, 128, 1024, [(0, 512)]), (128, 64, 2000, [(0, 64), (128, 1984)]),
+    (128, 64, 8000, [(0, 4032)]), (64, 64, 8192, [(0, 4608)]), (128, 128, 12000, [(256, 11904)]), (64, 32, 12000, [(0, 64), (96, 12000)]),
+    (128, 16, 300, [(0, 300)])])
+def test_attention_over_stretches_of_zeros(size, page, length, places, new):
+    """Tokens whose values are zero have the scale 0 and take their share of the softmax all the same."""
+    s = Served([length, 77], [new, new], 1, size, page, 'f16', heads=4)
+    nothing(s, 0, places)
+    out = s.attention()
+    runtime.token_check()
+    check_attention(s, out)
+
+
+@pytest.mark.parametrize('lengths', [[256] * 3, [600] * 40, [2047] * 80])
+def test_attention_over_zeros_in_every_split(lengths):
+    """Zeros over the first half of each of many sequences, so that the tokens are cut into few streams."""
+    s = Served(lengths, [1] * len(lengths), 8, 64, 64, 'bf16', heads=8, one_each=True)
+    for b, n in enumerate(lengths):
+        nothing(s, b, [(0, n // 2 // 64 * 64)])
+    out = s.attention()
+    runtime.token_check()
+    check_attention(s, out)
+
+
+@pytest.mark.parametrize('new', [1, 40, 300])
+@pytest.mark.parametrize('power', [-90, -60, 60, 110, 120])
+def test_attention_values_of_any_size(power, new):
+    """Every scale of the values times a power of two: the outputs are times that power."""
+    s = Served([700, 77], [new, min(new, 77)], 2, 128, 64, 'bf16', heads=8)
+    s.v_scales.mul_(2.0 ** power)
+    out = s.attention()
+    runtime.token_check()
+    s.v_scales.mul_(2.0 ** -power)
+    real = out[:s.tokens].double() * 2.0 ** -power
+    check_attention(s, torch.cat([real, out[s.tokens:].double()]))
+
+
+@pytest.mark.parametrize('new', [1, 40])
+def test_attention_values_of_nearly_nothing_beside_others(new):
+    """Scales of 2^-97 take their share of the softmax as scales of zero do."""
+    s = Served([3000, 77], [new, new], 1, 128, 64, 'f16', heads=4)
+    s.v_scales[s.table[0][:40]] = 2.0 ** -97
+    out = s.attention()
+    runtime.token_check()
+    check_attention(s, out)
