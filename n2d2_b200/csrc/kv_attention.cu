@@ -62,8 +62,10 @@ __device__ __forceinline__ float float_of(unsigned x, float by) { return fmaf(__
 
 static constexpr int ROWS_BLOCK = 128, ROWS_GROUP = 192;
 static constexpr int ROWS_FLUSH = 512;          // blocks whose sums stay within 32 bits: 512 x 128 x 255 x 128 < 2^31
-static constexpr float ROWS_ONE = 0x1p23f;      // the whole number of a probability of 1: 2^8 times as much still fits 32 bits
-static constexpr float ROWS_ROOM = 8.0f;        // powers of two that a score may be above the maximum before that moves
+// The whole number of a probability of 1, and the powers of two that a score may be above the maximum before that moves: 2^32, the most there can be, is taken as
+// 2^32 - 1.  The bits go to the small ones and not to the room: a probability is off by at most 2^-29 of the largest, so that the tokens beside one that takes 0.999 of
+// a row and holds zeros keep their bits (with 2^23 for 1 they were off by up to a quarter).
+static constexpr float ROWS_ONE = 0x1p28f, ROWS_ROOM = 4.0f;
 static constexpr float ROWS_NONE = -3.0e38f;    // the maximum of nothing
 // R: rows of a tile (4, 8 or 16); GROUPS: streams of tokens in a block
 template <int D, int R, int GROUPS> struct RowsSmem {

@@ -715,3 +715,35 @@ def test_attention_values_of_nearly_nothing_beside_others(new):
     out = s.attention()
     runtime.token_check()
     check_attention(s, out)
+
+
+@pytest.mark.parametrize('share', [0.9, 0.99, 0.999])
+@pytest.mark.parametrize('size, length, new, batch', [(64, 3000, 1, 1), (128, 3000, 2, 1), (64, 500, 4, 40), (128, 1800, 1, 160), (64, 4000, 2, 160)])
+def test_attention_of_single_tokens_beside_one_of_nothing(size, length, new, batch, share):
+    """A first token that takes nearly all of a row and holds zeros: what the others give is as exact as without it."""
+    s = Served([length] * batch, [new] * batch, 1, size, 64, 'f16', heads=4)
+    # the first key stands along the queries, the others across them: equal scores but for a little
+    s.q.copy_(torch.where(torch.arange(size, device='cuda') < size // 2, 1.0, 0.01 * normal(size, g=s.g)).half())
+    first = [row[0] for row in s.table]
+    s.k[:, :, :, :size // 2] = 0
+    s.k_scales.fill_(0.02)
+    s.k[first, :, 0, :size // 2], s.k[first, :, 0, size // 2:] = 100, 0
+    s.v[first, :, 0] = 0
+    s.v_scales.fill_(13.0)
+    scale = math.log(share / (1 - share) * length) / (100 * 0.02 * (size // 2))
+    out = s.attention(scale=scale, causal=False)
+    runtime.token_check()
+    for b in {0, batch // 2, batch - 1}:
+        used = s.table[b][:-(-length // 64)]
+        q, got = s.q[b * new:(b + 1) * new].double(), out[b * new:(b + 1) * new].double()
+        k = (s.k[used, 0].double() * s.k_scales[used, 0].double()[:, None, None]).flatten(0, 1)[:length]
+        v = (s.v[used, 0].double() * s.v_scales[used, 0].double()[:, None, None]).flatten(0, 1)[:length]
+        p = torch.softmax(q @ k.T * scale, 2)
+        want = p @ v
+        # scores as in check_attention (queries of 22 bits are exact here); 2^-22 of each exponential and of the scale's logarithm, sums in 32 bits; a
+        # probability is off by 2^-29 of the largest, half the step of a whole number of which the largest has 2^28
+        delta = (q.abs() @ k.abs().T * scale).amax(2, keepdim=True) * (size + 8) * 2 * U
+        relative = 2 * delta + 4 * 2.0 ** -21 + (length / 128 + 100) * U
+        bound = relative * (p @ v.abs()) + 2.0 ** -29 * p.amax(2, keepdim=True) * v.abs().sum(0) + half_step('f16') * want.abs() * 1.01 + 2.0 ** -25
+        off = (got - want).abs()
+        assert (off <= bound).all(), (b, float((off - bound).max()), float((off / want.abs().mean()).max()))
