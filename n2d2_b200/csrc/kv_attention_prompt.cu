@@ -392,6 +392,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_attention_prompt_kernel(cons
                         const float raised = ceilf(best) - PR_BITS, fade = !moves ? 1.0f : (top == -INFINITY ? 0.0f : __int_as_float((127 + (int)fmaxf(top - raised, -127.0f)) << 23));
                         if (moves) top = raised;
                         sum *= fade;
+                        tc_wait_st();       // what the quarters before stored: only this orders the loads behind it
                         const __half2 fade2 = __float2half2_rn(fade);
 #pragma unroll 1
                         for (int c = 0; c < 16 * q; c += 16) {        // this block's probabilities so far

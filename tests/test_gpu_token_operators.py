@@ -747,3 +747,25 @@ def test_attention_of_single_tokens_beside_one_of_nothing(size, length, new, bat
         bound = relative * (p @ v.abs()) + 2.0 ** -29 * p.amax(2, keepdim=True) * v.abs().sum(0) + half_step('f16') * want.abs() * 1.01 + 2.0 ** -25
         off = (got - want).abs()
         assert (off <= bound).all(), (b, float((off - bound).max()), float((off / want.abs().mean()).max()))
+
+
+@pytest.mark.parametrize('order', ['rising', 'falling', 'jumping', 'rising by little'])
+@pytest.mark.parametrize('size, page, heads, new, batch', [(128, 16, 16, 400, 1), (64, 32, 16, 1000, 1), (128, 16, 8, 300, 20), (64, 16, 4, 600, 40)])
+def test_attention_of_many_rows_whose_maxima_move_within_a_step(size, page, heads, new, batch, order):
+    """Scores that change every 16 or 32 tokens of a step of 128, by far more (or by about as much) as leaves the maximum where it is: what the tokens before gave
+    is rescaled again and again, inside the step and in the output so far.  Tokens over clusters of 4 and of 2 blocks, and undivided."""
+    length = 1000
+    s = Served([length] * batch, [new] * batch, 1, size, page, 'bf16', heads=heads)
+    s.q.copy_(s.q[:1, :1].sign())
+    s.k.copy_((s.q[0, 0] * 100).to(torch.int8))
+    steps = -(-length // page)
+    rise = torch.arange(steps, device='cuda') * (3.0 if order == 'rising by little' else 14.0)
+    if order == 'falling':
+        rise = rise.flip(0)
+    if order == 'jumping':
+        rise = rise[torch.randperm(steps, device='cuda', generator=s.g)]
+    for row in s.table:
+        s.k_scales[row[:steps]] = (rise / (100 * size ** 0.5))[:, None]
+    out = s.attention(causal=False)
+    runtime.token_check()
+    check_attention(s, out, causal=False)
