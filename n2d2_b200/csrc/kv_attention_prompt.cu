@@ -103,13 +103,26 @@ __device__ __forceinline__ float max_of(float a, float b, float c)
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
+__device__ __forceinline__ Pair mul_pair(Pair a, Pair b)
+{
+    Pair d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+// The larger one; no number if either is none
+__device__ __forceinline__ float max_or_nan(float a, float b)
+{
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
 // 2^x for x up to 14 without the exponential unit, which a quarter of the probabilities is kept from (it takes 8 cycles for a warp's 32 and would bound
 // the kernel): x = n + f with n whole, 2^f on [-1/2, 1/2] by the polynomial of degree 4 with the smallest relative error (2.6e-6, from an exchange
-// iteration), n added to its exponent.  Below 2^-126 the result is that.
+// iteration), times the number with the exponent n.  That is 0 from n = -127 down, and what is no number stays that, whatever the bits of its n make of the factor.
 __device__ __forceinline__ Pair exp2_pair(Pair x)
 {
     const float2 v = both_of(x);
-    x = pair_of(fmaxf(v.x, -126.0f), fmaxf(v.y, -126.0f));
+    x = pair_of(max_or_nan(v.x, -127.0f), max_or_nan(v.y, -127.0f));
     const Pair r = add_pair(x, pair_of(12582912.0f, 12582912.0f));      // 1.5 * 2^23: n in the lowest bits
     const Pair f = fma_pair(add_pair(r, pair_of(-12582912.0f, -12582912.0f)), pair_of(-1.0f, -1.0f), x);
     Pair p = pair_of(0.009570102207362652f, 0.009570102207362652f);
@@ -117,8 +130,8 @@ __device__ __forceinline__ Pair exp2_pair(Pair x)
     p = fma_pair(p, f, pair_of(0.240247443318367f, 0.240247443318367f));
     p = fma_pair(p, f, pair_of(0.6931217908859253f, 0.6931217908859253f));
     p = fma_pair(p, f, pair_of(0.9999992847442627f, 0.9999992847442627f));
-    const float2 y = both_of(p), n = both_of(r);
-    return pair_of(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(n.x) << 23)), __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(n.y) << 23)));
+    const float2 n = both_of(r);
+    return mul_pair(p, pair_of(__uint_as_float((__float_as_uint(n.x) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(n.y) << 23) + 0x3f800000u)));
 }
 template <bool M> struct Masked { static constexpr bool value = M; };
 
@@ -332,7 +345,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_attention_prompt_kernel(cons
 #pragma unroll
                 for (int x = 0; x < 8; ++x) largest = max(largest, magnitude(f[x]));
             }
-            // a power of two brings the row's largest value into [1, 4); the sign of the scale goes with it
+            // a power of two brings the row's largest value into [1, 4); the sign of the scale goes with it.
             const int exponent = min((int)(largest >> 23), 253);
             const bool scaled = exponent > 0 && largest < 0x7f800000u;
             const float up = copysignf(scaled ? __int_as_float((254 - exponent) << 23) : 1.0f, a.scale_log2);

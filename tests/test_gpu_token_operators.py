@@ -769,3 +769,39 @@ def test_attention_of_many_rows_whose_maxima_move_within_a_step(size, page, head
     out = s.attention(causal=False)
     runtime.token_check()
     check_attention(s, out, causal=False)
+
+
+@pytest.mark.parametrize('window', [1, 2, 3, 15, 16, 17, 40])
+@pytest.mark.parametrize('size, page', [(64, 16), (128, 16), (128, 64)])
+@pytest.mark.parametrize('which', ['k_scales', 'v_scales', 'table'])
+def test_attention_a_window_that_ends_in_a_poisoned_page(which, size, page, window):
+    """Every place of a page at a window's lower edge: no number for those who see the page, the same bits for all others."""
+    new = 1000 if window < 40 else 40
+    s = Served([1100], [new], 2, size, page, 'bf16', heads=8)
+    clean = s.attention(window=window)
+    bad = 1 + 1080 // page // 2 * 2 - 2
+    bad = min(bad, 1099 // page)
+    if which == 'table':
+        s.device_table[0, bad] = s.pages
+    else:
+        getattr(s, which)[s.table[0][bad]] = math.nan
+    out = s.attention(window=window)
+    runtime.token_check()
+    position = torch.arange(1100 - new, 1100, device='cuda')
+    sees = (position >= bad * page) & (position - window < (bad + 1) * page - 1)
+    assert sees.any()
+    assert out[:new][sees].isnan().all()
+    assert torch.equal(out[:new][~sees], clean[:new][~sees])
+
+
+@pytest.mark.parametrize('window', [1, 2, 5])
+@pytest.mark.parametrize('new', [16, 1000])
+def test_attention_queries_that_are_no_number_in_narrow_windows(new, window):
+    s = Served([1000], [new], 2, 128, 64, 'bf16', heads=8)
+    clean = s.attention(window=window)
+    s.q[:, [1, 6], 7] = math.nan
+    out = s.attention(window=window)
+    runtime.token_check()
+    assert out[:new, [1, 6]].isnan().all()
+    keep = [0, 2, 3, 4, 5, 7]
+    assert torch.equal(out[:new, keep], clean[:new, keep])
