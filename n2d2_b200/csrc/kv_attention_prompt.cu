@@ -345,10 +345,11 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_attention_prompt_kernel(cons
 #pragma unroll
                 for (int x = 0; x < 8; ++x) largest = max(largest, magnitude(f[x]));
             }
-            // a power of two brings the row's largest value into [1, 4); the sign of the scale goes with it.
+            // a power of two brings the row's largest value into [1, 4); the sign of the scale goes with it.  A row that is not finite becomes no numbers
+            // altogether: a score of -inf would count as one that is not seen.
             const int exponent = min((int)(largest >> 23), 253);
-            const bool scaled = exponent > 0 && largest < 0x7f800000u;
-            const float up = copysignf(scaled ? __int_as_float((254 - exponent) << 23) : 1.0f, a.scale_log2);
+            const bool finite = largest < 0x7f800000u, scaled = exponent > 0 && finite;
+            const float up = finite ? copysignf(scaled ? __int_as_float((254 - exponent) << 23) : 1.0f, a.scale_log2) : __int_as_float(0x7fffffff);
             row_scale = fabsf(a.scale_log2) * (scaled ? __int_as_float(exponent << 23) : 1.0f);
 #pragma unroll 4
             for (int e = 0; e < D / 8; ++e) {

@@ -805,3 +805,18 @@ def test_attention_queries_that_are_no_number_in_narrow_windows(new, window):
     assert out[:new, [1, 6]].isnan().all()
     keep = [0, 2, 3, 4, 5, 7]
     assert torch.equal(out[:new, keep], clean[:new, keep])
+
+
+@pytest.mark.parametrize('what', [math.inf, -math.inf])
+@pytest.mark.parametrize('window', [1, 2, 5, 0])
+@pytest.mark.parametrize('new', [16, 1000])
+def test_attention_queries_that_are_infinite(new, window, what):
+    """An infinite query gives no numbers, as the few rows have it, not what one that sees nothing gives where all its scores are -inf."""
+    s = Served([1000], [new], 2, 128, 64, 'bf16', heads=8)
+    clean = s.attention(window=window)
+    s.q[:, 6, 7] = what
+    out = s.attention(window=window)
+    runtime.token_check()
+    assert out[:new, 6].isnan().all()
+    keep = [0, 1, 2, 3, 4, 5, 7]
+    assert torch.equal(out[:new, keep], clean[:new, keep])
