@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(512) rmsnorm_quantize_kernel(const NormArgs a)
     float step = __uint_as_float(top) * TOKEN_STEP, inverse = 1.0f / step;
     if (step <= TOKEN_TINY) step = inverse = 0.0f;
     if (top >= 0x7f800000u) step = __int_as_float(0x7fffffff);
-    if (threadIdx.x == 0) a.scales[row] = step * rsqrtf(sum / (float)a.columns + a.eps);
+    if (threadIdx.x == 0) a.scales[row] = step == 0.0f ? 0.0f : step * rsqrtf(sum / (float)a.columns + a.eps);
     if (ITER) {
 #pragma unroll
         for (int k = 0; k < ITER; ++k) {

@@ -820,3 +820,19 @@ def test_attention_queries_that_are_infinite(new, window, what):
     assert out[:new, 6].isnan().all()
     keep = [0, 1, 2, 3, 4, 5, 7]
     assert torch.equal(out[:new, keep], clean[:new, keep])
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('columns', [64, 77, 4096, 20000])
+@pytest.mark.parametrize('residual', [False, True])
+def test_norm_rows_of_zeros_without_eps(columns, residual, dtype):
+    """A scale of nothing is 0, whatever 0 / 0 is: a padded row, and one whose weights are zero where it is not."""
+    x = torch.zeros((3, columns), device='cuda', dtype=TYPES[dtype])
+    x[1, :5] = 2
+    w = torch.ones(columns, device='cuda', dtype=TYPES[dtype])
+    w[:5] = 0
+    codes, scales = torch.full((3, columns), 5, dtype=torch.int8, device='cuda'), torch.full((3,), 9.0, device='cuda')
+    r, total = torch.zeros_like(x), torch.ones_like(x)
+    runtime.rmsnorm_quantize(x.data_ptr(), 3, columns, w.data_ptr(), codes.data_ptr(), scales.data_ptr(), r.data_ptr() if residual else None,
+                             total.data_ptr() if residual else None, dtype=dtype, eps=0.0)
+    assert (scales == 0).all() and (codes == 0).all()
