@@ -365,8 +365,8 @@ int n2d2b_token_selftest_wait_timeout(int device, unsigned limit_us, n2d2b_strea
 /* Root-mean-square norm with 8-bit output, a scale for each row:
  *   h = x + residual, rounded to dtype (h = x without a residual); u = h * weight (32 bits)
  *   step = max|u| * (1/127);  codes = round(u * (1/step));  scales = step / sqrt(mean(h^2) + eps)
- * so codes * scales is h * weight / sqrt(mean(h^2) + eps) rounded to 255 levels.  The squares are summed in 32 bits: h^2 has to stay
- * below 2^127. */
+ * so codes * scales is h * weight / sqrt(mean(h^2) + eps) rounded to 255 levels.  The squares are summed in 32 bits, on a scale of their own where
+ * they would leave those: any finite h does whose products with the weight are finite in 32 bits. */
 typedef struct n2d2b_norm {
     int32_t dtype;             /* of x, residual, total and weight: N2D2B_F32, N2D2B_F16 or N2D2B_BF16 */
     int32_t rows, columns;

@@ -836,3 +836,27 @@ def test_norm_rows_of_zeros_without_eps(columns, residual, dtype):
     runtime.rmsnorm_quantize(x.data_ptr(), 3, columns, w.data_ptr(), codes.data_ptr(), scales.data_ptr(), r.data_ptr() if residual else None,
                              total.data_ptr() if residual else None, dtype=dtype, eps=0.0)
     assert (scales == 0).all() and (codes == 0).all()
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+@pytest.mark.parametrize('columns', [1, 77, 512, 4096, 20000])
+@pytest.mark.parametrize('power', [-90, -75, -62, 50, 61, 63, 64, 100, 120])
+@pytest.mark.parametrize('form', ['plain', 'weight', 'residual', 'in place'])
+def test_norm_of_rows_of_any_size(form, power, columns, dtype):
+    """Rows whose squares leave 32 bits on either side, without eps; beside them one of ordinary size."""
+    g, t = gen(columns + 200 + power), TYPES[dtype]
+    x = normal(3, columns, g=g).abs().add_(0.1).mul_(torch.where(normal(3, columns, g=g) < 0, -1.0, 1.0)).to(t)
+    x[0] *= 2.0 ** power
+    x[1] *= 2.0 ** power
+    x[1, columns // 2:] = 0
+    if columns == 1:
+        x[1] = 2.0 ** power
+    w = (1 + 0.3 * normal(columns, g=g)).to(t) if form == 'weight' else None
+    r = torch.zeros_like(x)
+    total = x if form == 'in place' else torch.ones_like(x)
+    more = form in ('residual', 'in place')
+    h = x.clone()
+    codes, scales = torch.zeros((3, columns), dtype=torch.int8, device='cuda'), torch.zeros(3, device='cuda')
+    runtime.rmsnorm_quantize(x.data_ptr(), 3, columns, w.data_ptr() if w is not None else None, codes.data_ptr(), scales.data_ptr(),
+                             r.data_ptr() if more else None, total.data_ptr() if more else None, dtype=dtype, eps=0.0)
+    check_norm(h, w, codes, scales, dtype, 0.0)
