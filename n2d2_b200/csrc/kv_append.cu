@@ -43,7 +43,8 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvArgs c, const T*
         const int at = threadIdx.x + i * 256;
         if (at < n) kept[i] = *reinterpret_cast<const uint4*>(x + (size_t)(at / PER) * stride + (at % PER) * 8);
     }
-    const float before = lo > p * page ? *scale : 0.0f;
+    // (a scale that counts as zero is 0 here: the reciprocals of such leave 32 bits)
+    const float held = lo > p * page ? *scale : 0.0f, before = held <= TOKEN_TINY ? 0.0f : held;
 #pragma unroll
     for (int i = 0; i < KEEP; ++i) {
         const int at = threadIdx.x + i * 256;
@@ -74,7 +75,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvArgs c, const T*
             *reinterpret_cast<uint2*>(codes + (size_t)(lo - p * page) * D + (size_t)at * 8) = make_uint2(pack_codes(v, inverse), pack_codes(v + 4, inverse));
         }
     }
-    if (lo > p * page && after != before) {
+    if (lo > p * page && after != held) {
         const float ratio = after > 0.0f ? before / after : 0.0f;
         const int old = (lo - p * page) * D / 4;
         for (int i = threadIdx.x; i < old; i += 256) {

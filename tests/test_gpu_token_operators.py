@@ -860,3 +860,22 @@ def test_norm_of_rows_of_any_size(form, power, columns, dtype):
     runtime.rmsnorm_quantize(x.data_ptr(), 3, columns, w.data_ptr() if w is not None else None, codes.data_ptr(), scales.data_ptr(),
                              r.data_ptr() if more else None, total.data_ptr() if more else None, dtype=dtype, eps=0.0)
     check_norm(h, w, codes, scales, dtype, 0.0)
+
+
+@pytest.mark.parametrize('held', [1e-45, 1e-40, 2.0 ** -127, 2.0 ** -110, 2.0 ** -100])
+@pytest.mark.parametrize('fresh', [0.0, 2.0 ** -96, 1.0])
+def test_append_onto_a_page_of_nearly_nothing(held, fresh):
+    """A scale up to 2^-100 is 0, the one a page holds too: its codes become 0, as those of new values that small."""
+    s = Served([20], [3], 2, 64, 32, 'bf16')
+    s.k_scales.fill_(held)
+    s.new_k[:] = fresh * normal(s.joint.shape[0], 2, 64, g=s.g).clamp(-1, 1).bfloat16()
+    k = s.k.clone()
+    s.append()
+    number = s.table[0][0]
+    assert (s.k[number, :, :17] == 0).all()
+    if fresh < 1:
+        assert (s.k_scales[number] == 0).all() and (s.k[number, :, 17:20] == 0).all()
+    else:
+        x = s.new_k[:3].double().transpose(0, 1)
+        assert ((s.k[number, :, 17:20] * s.k_scales[number].double()[:, None, None] - x).abs() <= s.k_scales[number].double()[:, None, None] * 0.501).all()
+    assert torch.equal(s.k[number, :, 20:], k[number, :, 20:])
