@@ -92,8 +92,9 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvArgs c, const T*
 template <typename T>
 static cudaError_t launch_append(const KvArgs& c, const void* k, const void* v, long long stride, int page, int head_size, int sequences, cudaStream_t s)
 {
-    // new tokens of a sequence lie in at most this many pages
-    const dim3 grid((unsigned)(((long long)c.max_new + page - 2) / page + 1), (unsigned)c.heads, (unsigned)(2 * sequences));
+    // new tokens of a sequence lie in at most this many pages, none behind its row of the table
+    const long long pages = ((long long)c.max_new + page - 2) / page + 1;
+    const dim3 grid((unsigned)(pages < c.row ? pages : c.row), (unsigned)c.heads, (unsigned)(2 * sequences));
     if (head_size == 64) return launch_token(kv_append_kernel<T, 64>, grid, 256, 0, 1, s, c, (const T*)k, (const T*)v, stride, page);
     return launch_token(kv_append_kernel<T, 128>, grid, 256, 0, 1, s, c, (const T*)k, (const T*)v, stride, page);
 }

@@ -59,7 +59,9 @@ static inline int kv_check(const n2d2b_kv_cache* cache, const n2d2b_kv_batch* ba
     a.table = batch->page_table; a.lengths = batch->lengths; a.starts = batch->starts;
     a.nb_pages = cache->nb_pages; a.heads = cache->nb_heads; a.row = batch->pages_per_sequence;
     a.nb_tokens = batch->nb_tokens;
+    // a bound may be as loose as the caller likes: no sequence has more new tokens than the call has rows, and blocks are launched for no more
     a.max_new = batch->starts ? batch->max_new : (batch->max_new < 1 ? batch->max_new : 1);
+    if (a.max_new > batch->nb_tokens) a.max_new = batch->nb_tokens;
     return 0;
 }
 

@@ -879,3 +879,20 @@ def test_append_onto_a_page_of_nearly_nothing(held, fresh):
         x = s.new_k[:3].double().transpose(0, 1)
         assert ((s.k[number, :, 17:20] * s.k_scales[number].double()[:, None, None] - x).abs() <= s.k_scales[number].double()[:, None, None] * 0.501).all()
     assert torch.equal(s.k[number, :, 20:], k[number, :, 20:])
+
+
+@pytest.mark.parametrize('lengths, news', [([70, 33, 200], [1, 9, 40]), ([64], [64])])
+def test_a_loose_bound_of_new_tokens_changes_nothing(lengths, news):
+    s = Served(lengths, news, 2, 64, 16, 'bf16', heads=8)
+    tight = Served(lengths, news, 2, 64, 16, 'bf16', heads=8)
+    s.batch.desc.max_new = 2 ** 31 - 1
+    tight.batch.desc.max_new = s.tokens
+    k, v, ks, vs = s.k.clone(), s.v.clone(), s.k_scales.clone(), s.v_scales.clone()
+    s.append()
+    tight.append()
+    out, want = s.attention(), tight.attention()
+    runtime.token_check()
+    check_append(s, k, s.k, ks, s.k_scales, s.new_k)
+    check_append(s, v, s.v, vs, s.v_scales, s.new_v)
+    check_attention(s, out)
+    assert torch.equal(out, want) and torch.equal(s.k, tight.k) and torch.equal(s.v_scales, tight.v_scales)

@@ -139,3 +139,14 @@ def test_no_fallback_without_a_device():
         pytest.skip('a GPU is present')
     for rc in (norm(), matmul(), append(), attention(), runtime.load().n2d2b_token_check(0, None)):
         refused(rc, 'device 0 is not usable', CUDA)
+
+
+def test_a_loose_bound_of_new_tokens_is_no_reason_to_refuse():
+    """max_new only bounds: a call of few rows is as large as its rows."""
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip('a GPU is present')
+    loose = dict(max_new=2**31 - 1, nb_tokens=7, starts=BASE, nb_sequences=32767, nb_heads=64, nb_query_heads=512)
+    refused(attention(**loose), 'device 0 is not usable', CUDA)
+    loose.pop('nb_query_heads')
+    refused(append(**loose), 'device 0 is not usable', CUDA)
