@@ -418,7 +418,7 @@ typedef struct n2d2b_kv_cache {
  * makes the outputs of the queries that see it not a number. */
 typedef struct n2d2b_kv_batch {
     int32_t nb_sequences;
-    int32_t pages_per_sequence;  /* entries of a row of page_table */
+    int32_t pages_per_sequence;  /* entries of a row of page_table; times page_tokens at most 2^31 - 512 */
     int32_t nb_tokens;           /* rows of the call's tensors */
     int32_t max_new;             /* bound of a sequence's new tokens */
     const int32_t* page_table;   /* [nb_sequences][pages_per_sequence] */

@@ -50,8 +50,9 @@ static inline int kv_check(const n2d2b_kv_cache* cache, const n2d2b_kv_batch* ba
         return set_error(N2D2B_ERR_INVALID, "invalid batch: %d sequences, %d tokens, at most %d new, %d pages a sequence", batch->nb_sequences,
                          batch->nb_tokens, batch->max_new, batch->pages_per_sequence);
     if (batch->nb_sequences > 32767) return set_error(N2D2B_ERR_TOO_LARGE, "nb_sequences = %d exceeds 32767", batch->nb_sequences);
-    if (batch->pages_per_sequence > 2147483647 / cache->page_tokens - 1)
-        return set_error(N2D2B_ERR_TOO_LARGE, "pages_per_sequence x page_tokens exceeds 2^31 - 1");
+    // (kernels count in steps of 128 tokens and look two steps ahead)
+    if (batch->pages_per_sequence > (2147483647 - 511) / cache->page_tokens)
+        return set_error(N2D2B_ERR_TOO_LARGE, "pages_per_sequence x page_tokens exceeds 2^31 - 512");
     if (batch->nb_sequences > 0 && (!batch->page_table || !batch->lengths)) return set_error(N2D2B_ERR_INVALID, "page_table and lengths must not be NULL");
     if (!token_aligned(batch->page_table, 4) || !token_aligned(batch->lengths, 4) || !token_aligned(batch->starts, 4))
         return set_error(N2D2B_ERR_INVALID, "page_table, lengths and starts must start on 4 bytes");

@@ -150,3 +150,14 @@ def test_a_loose_bound_of_new_tokens_is_no_reason_to_refuse():
     refused(attention(**loose), 'device 0 is not usable', CUDA)
     loose.pop('nb_query_heads')
     refused(append(**loose), 'device 0 is not usable', CUDA)
+
+
+@pytest.mark.parametrize('page', [16, 32, 64, 128])
+def test_positions_stay_in_32_bits(page):
+    """The last step of 128 tokens of the longest row of pages, and the two that are looked ahead, end below 2^31."""
+    most = (2**31 - 512) // page
+    for call in (append, attention):
+        refused(call(page_tokens=page, nb_pages=1, nb_heads=1, nb_query_heads=1, pages_per_sequence=most + 1) if call is attention else
+                call(page_tokens=page, nb_pages=1, nb_heads=1, pages_per_sequence=most + 1), '2^31 - 512', TOO_LARGE)
+    capacity = most * page
+    assert (capacity + 127) // 128 * 128 + 2 * 128 <= 2**31
