@@ -366,7 +366,9 @@ int n2d2b_token_selftest_wait_timeout(int device, unsigned limit_us, n2d2b_strea
  *   h = x + residual, rounded to dtype (h = x without a residual); u = h * weight (32 bits)
  *   step = max|u| * (1/127);  codes = round(u * (1/step));  scales = step / sqrt(mean(h^2) + eps)
  * so codes * scales is h * weight / sqrt(mean(h^2) + eps) rounded to 255 levels.  The squares are summed in 32 bits, on a scale of their own where
- * they would leave those: any finite h does whose products with the weight are finite in 32 bits. */
+ * they would leave those: any finite h does whose products with the weight are finite in 32 bits.
+ * With skip_norm the scales are step alone and codes * scales is h * weight: the input of a product that has no norm ahead of it.  Start from a
+ * description of zeros. */
 typedef struct n2d2b_norm {
     int32_t dtype;             /* of x, residual, total and weight: N2D2B_F32, N2D2B_F16 or N2D2B_BF16 */
     int32_t rows, columns;
@@ -378,6 +380,7 @@ typedef struct n2d2b_norm {
     int8_t* codes;
     float* scales;             /* rows entries */
     int64_t x_stride, residual_stride, total_stride, codes_stride;
+    int32_t skip_norm;         /* 1: codes and scales of h * weight itself (eps has no meaning); 0: of its norm */
 } n2d2b_norm;
 int n2d2b_rmsnorm_quantize(int device, const n2d2b_norm* norm, n2d2b_stream stream);
 

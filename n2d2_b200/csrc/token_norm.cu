@@ -2,7 +2,7 @@
 //
 //   h = round(x + r)          stored in the inputs' type
 //   u = h * w                 32 bits
-//   s = max |u| / 127         code = round(u / s), scale = s / sqrt(mean(h^2) + eps)
+//   s = max |u| / 127         code = round(u / s), scale = s / sqrt(mean(h^2) + eps), or s alone where no norm is wanted
 //
 // The factor 1 / sqrt(...) is the same for a whole row, so it cancels out of the codes: they are taken of u, do not depend on the
 // order in which the squares are summed, and the row's sum and maximum come out of one pass and one reduction.
@@ -67,7 +67,7 @@ struct NormArgs {
     int8_t* codes;
     float* scales;
     long long x_stride, residual_stride, total_stride, codes_stride;
-    int columns;
+    int columns, skip_norm;
     float eps, least;       // least: sums of squares below it have lost some that count beside eps
 };
 
@@ -190,8 +190,8 @@ __global__ void __launch_bounds__(512, ITER < 4 || VEC == 1 ? 4 : VEC == 4 ? 3 :
     if (step <= TOKEN_TINY) step = inverse = 0.0f;
     if (top >= 0x7f800000u) step = __int_as_float(0x7fffffff);
     // squares that left 32 bits: values above 2^63 or so, or below 2^-63 with no eps to speak of
-    const bool large = step > 0.0f && sum == INFINITY, small = step > 0.0f && sum < a.least;
-    if (threadIdx.x == 0) a.scales[row] = step == 0.0f ? 0.0f : large || small ? step : step * rsqrtf(sum / (float)a.columns + a.eps);
+    const bool large = step > 0.0f && sum == INFINITY && !a.skip_norm, small = step > 0.0f && sum < a.least;
+    if (threadIdx.x == 0) a.scales[row] = step == 0.0f ? 0.0f : large || small || a.skip_norm ? step : step * rsqrtf(sum / (float)a.columns + a.eps);
     if (ITER) {
 #pragma unroll
         for (int k = 0; k < ITER; ++k) {
@@ -258,7 +258,8 @@ extern "C" int n2d2b_rmsnorm_quantize(int device, const n2d2b_norm* norm, n2d2b_
     a.x = d.x; a.residual = d.residual; a.weight = d.weight; a.total = d.total; a.codes = d.codes; a.scales = d.scales;
     a.columns = d.columns;
     a.eps = d.eps;
-    a.least = d.eps < 0x1p-60f ? (0x1p-60f - d.eps) * (float)d.columns : 0.0f;
+    a.skip_norm = d.skip_norm;
+    a.least = d.eps < 0x1p-60f && !d.skip_norm ? (0x1p-60f - d.eps) * (float)d.columns : 0.0f;
     a.x_stride = d.x_stride ? d.x_stride : d.columns;
     a.residual_stride = d.residual_stride ? d.residual_stride : d.columns;
     a.total_stride = d.total_stride ? d.total_stride : d.columns;

@@ -60,7 +60,7 @@ class TensorInfo(C.Structure):
 class Norm(C.Structure):
     _fields_ = [('dtype', C.c_int32), ('rows', C.c_int32), ('columns', C.c_int32), ('eps', C.c_float), ('x', C.c_void_p), ('residual', C.c_void_p),
                 ('total', C.c_void_p), ('weight', C.c_void_p), ('codes', C.c_void_p), ('scales', C.c_void_p), ('x_stride', C.c_int64),
-                ('residual_stride', C.c_int64), ('total_stride', C.c_int64), ('codes_stride', C.c_int64)]
+                ('residual_stride', C.c_int64), ('total_stride', C.c_int64), ('codes_stride', C.c_int64), ('skip_norm', C.c_int32)]
 
 
 class Matmul(C.Structure):
@@ -398,10 +398,11 @@ def _float_type(dtype):
 
 
 def rmsnorm_quantize(x_ptr, rows, columns, weight_ptr, codes_ptr, scales_ptr, residual_ptr=None, total_ptr=None, dtype='bf16', eps=1e-6,
-                     x_stride=0, residual_stride=0, total_stride=0, codes_stride=0, device=0, stream=0):
-    """Root-mean-square norm of x (+ residual, the sum into total) as int8 codes with a scale for each row; see n2d2b_rmsnorm_quantize."""
+                     x_stride=0, residual_stride=0, total_stride=0, codes_stride=0, device=0, stream=0, skip_norm=False):
+    """Root-mean-square norm of x (+ residual, the sum into total) as int8 codes with a scale for each row, with skip_norm x (+ residual) itself; see
+    n2d2b_rmsnorm_quantize."""
     d = Norm(_float_type(dtype), rows, columns, eps, x_ptr, residual_ptr, total_ptr, weight_ptr, codes_ptr, scales_ptr, x_stride,
-             residual_stride, total_stride, codes_stride)
+             residual_stride, total_stride, codes_stride, 1 if skip_norm else 0)
     check(load().n2d2b_rmsnorm_quantize(device, C.byref(d), stream))
 
 

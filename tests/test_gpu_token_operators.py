@@ -896,3 +896,76 @@ def test_a_loose_bound_of_new_tokens_changes_nothing(lengths, news):
     check_append(s, v, s.v, vs, s.v_scales, s.new_v)
     check_attention(s, out)
     assert torch.equal(out, want) and torch.equal(s.k, tight.k) and torch.equal(s.v_scales, tight.v_scales)
+
+
+# ------------------------------------------------------------------------------------------------ codes without a norm
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('columns, form', [(1, 'plain'), (77, 'residual'), (512, 'plain'), (4096, 'weight'), (4096, 'residual'), (20000, 'weight')])
+@pytest.mark.parametrize('power', [-60, 0, 70])
+def test_codes_without_a_norm(power, columns, form, dtype):
+    if dtype == 'f16' and power:
+        pytest.skip('16 bits do not hold them')
+    g, t = gen(columns), TYPES[dtype]
+    x, r = (normal(4, columns, g=g) * 2.0 ** power).to(t), (normal(4, columns, g=g) * 2.0 ** power).to(t)
+    x[2] = r[2] = 0
+    w = (1 + 0.3 * normal(columns, g=g)).to(t) if form == 'weight' else None
+    total = torch.ones_like(x)
+    codes, scales = torch.full((4, columns), 9, dtype=torch.int8, device='cuda'), torch.full((4,), 9.0, device='cuda')
+    more = form == 'residual'
+    runtime.rmsnorm_quantize(x.data_ptr(), 4, columns, w.data_ptr() if w is not None else None, codes.data_ptr(), scales.data_ptr(),
+                             r.data_ptr() if more else None, total.data_ptr() if more else None, dtype=dtype, eps=0.0, skip_norm=True)
+    h = (x.float() + r.float()).to(t) if more else x
+    if more:
+        assert torch.equal(total, h)
+    u = h.double() * (1.0 if w is None else w.double())
+    step = u.abs().amax(1) / 127
+    # a product and the constant in 32 bits; the codes as in check_norm
+    assert ((scales.double() - step).abs() <= step * 3 * U).all()
+    assert (scales[2] == 0) and (codes[2] == 0).all()
+    assert ((codes.double() - u / torch.where(step > 0, step, 1.0)[:, None]).abs() <= 0.5 + 127 * 5 * U).all()
+
+
+@pytest.mark.parametrize('lengths, news', [([70, 33, 1], [1, 1, 1]), ([200, 90], [70, 90])])
+def test_a_layer_against_the_layer_in_64_bits(lengths, news):
+    """Norm, joint projection, append, attention and the projection back, as a user chains them, against the same layer without any rounding.
+
+    What 8 bits cost: a rounding to a step s is noise of s / sqrt(12).  The largest of some hundred normal values is about 3.2 of their widths (of a page's 64 x 32, 3.7), so a
+    step is 3.2 / 127 = 2.5 % of the width and its noise 0.7 % (0.9 % of a page's values, and as much again where its scale grows under old codes).  A product
+    hands the relative noise of its input on as it is, and attention averages that of the values.  Three roundings one after the other: the normed input, keys and
+    values, attention's output: sqrt(0.7^2 + 2 * 0.9^2 + 0.7^2) = 1.6 %, 0.3 % of bf16 beside it.  Scores are of the order of 1, so that the keys' and queries' own noise moves them by
+    1 to 2 %, and the outputs by as much at most: 2.6 % in all.  A layer that takes another scale anywhere is off by tens of percent."""
+    s, args = make_layer(lengths, news)
+    x, residual, w_norm, w_joint, w_scales, w_out, w_out_scales, (codes, scales, total, codes2, scales2, out, back) = args
+    rows, width = x.shape
+    # a cache whose earlier tokens are of the size that the projection gives
+    s.k_scales.mul_(1.5)
+    s.v_scales.mul_(1.5)
+    held = [(s.k.double() * s.k_scales.double()[..., None, None]), (s.v.double() * s.v_scales.double()[..., None, None])]
+    joint = s.joint.shape[1]
+    runtime.rmsnorm_quantize(x.data_ptr(), rows, width, w_norm.data_ptr(), codes.data_ptr(), scales.data_ptr(), residual.data_ptr(), total.data_ptr(),
+                             dtype=s.dtype)
+    runtime.matmul_i8(codes.data_ptr(), scales.data_ptr(), w_joint.data_ptr(), w_scales.data_ptr(), s.joint.data_ptr(), rows, joint, width, dtype=s.dtype)
+    s.append()
+    s.attention(out)
+    runtime.rmsnorm_quantize(out.data_ptr(), rows, s.heads * s.size, None, codes2.data_ptr(), scales2.data_ptr(), dtype=s.dtype, skip_norm=True)
+    runtime.matmul_i8(codes2.data_ptr(), scales2.data_ptr(), w_out.data_ptr(), w_out_scales.data_ptr(), back.data_ptr(), rows, width, s.heads * s.size, dtype='f32')
+    runtime.token_check()
+
+    h = x.double() + residual.double()
+    n = h / torch.sqrt((h * h).mean(1, keepdim=True) + 1e-6) * w_norm.double()
+    j = n @ (w_joint.double() * w_scales.double()[:, None]).T
+    q, k, v = j.split([s.heads * s.size, s.kv_heads * s.size, s.kv_heads * s.size], 1)
+    attended = torch.zeros(rows, s.heads, s.size, dtype=torch.float64, device='cuda')
+    for b, (end, new) in enumerate(zip(lengths, news)):
+        used, at = s.table[b][:-(-end // s.page)], slice(s.starts[b], s.starts[b] + new)
+        full = []
+        for pool, fresh in zip(held, (k, v)):
+            t = pool[used].transpose(1, 2).flatten(0, 1)[:end].clone()          # [token][head][size]
+            t[end - new:] = fresh[at].unflatten(1, (s.kv_heads, s.size))
+            full.append(t.repeat_interleave(s.heads // s.kv_heads, 1))
+        scores = torch.einsum('thd,jhd->htj', q[at].unflatten(1, (s.heads, s.size)), full[0]) * s.size ** -0.5
+        hidden = torch.arange(end, device='cuda')[None] > torch.arange(end - new, end, device='cuda')[:, None]
+        attended[at] = torch.einsum('htj,jhd->thd', torch.softmax(scores.masked_fill(hidden, -math.inf), 2), full[1])
+    want = attended.flatten(1) @ (w_out.double() * w_out_scales.double()[:, None]).T
+    off = (back.double() - want).square().mean().sqrt() / want.square().mean().sqrt()
+    assert off <= 0.026, float(off)
