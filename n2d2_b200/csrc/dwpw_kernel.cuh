@@ -247,7 +247,6 @@ dwpw_i8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
     volatile int* const abort_flag = (volatile int*)(tmem_slot + 1);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const int lane = threadIdx.x & 31;
-    pdl_launch_dependents();
 
     if (warp == 0) {
         for (int i = lane; i < DP_BARS; i += 32) {
@@ -267,6 +266,7 @@ dwpw_i8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      ::"r"(smem_u32(tmem_slot)), "r"(a.tmem_cols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        pdl_launch_dependents();   // (only now: see there)
     }
     tc_fence_before();
     __syncthreads();

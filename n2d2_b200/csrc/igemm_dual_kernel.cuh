@@ -112,7 +112,6 @@ igemm_dual_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid
     const int lane = threadIdx.x & 31;
     constexpr int LAST_PRODUCERS = EPI_WARP0 + NUM_EPI_WARPS;
     const int producer = warp == 0 ? 0 : (warp >= LAST_PRODUCERS ? warp - LAST_PRODUCERS + 1 : -1);
-    pdl_launch_dependents();
 
     if (warp == 0) {
         const int nb = 2 * a.stages + 2 * MAX_ACC + 2;
@@ -138,6 +137,7 @@ igemm_dual_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      ::"r"(smem_u32(tmem_slot)), "r"(a.tmem_cols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        pdl_launch_dependents();   // (only now: see there)
     }
     tc_fence_before();
     __syncthreads();

@@ -41,7 +41,6 @@ igemm_pair_i8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __gr
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const int lane = threadIdx.x & 31;
     const int producer = warp == 0 ? 0 : (warp >= EPI_WARP0 + NUM_EPI_WARPS ? warp - (EPI_WARP0 + NUM_EPI_WARPS) + 1 : -1);
-    pdl_launch_dependents();
     if (threadIdx.x == 0) {
         for (int s = 0; s < PAIR_STAGES; ++s) {
             mbar_init(full0 + 8u * s, 1);
@@ -59,6 +58,7 @@ igemm_pair_i8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __gr
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        pdl_launch_dependents();   // (only now: see there)
     }
     tc_fence_before();
     __syncthreads();
@@ -637,7 +637,6 @@ igemm_split_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const int lane = threadIdx.x & 31;
-    pdl_launch_dependents();
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // (waited for before the first remote store)
 
     const int tile = (int)blockIdx.x / S, rank = (int)blockIdx.x % S;   // clusters are S consecutive CTAs
@@ -657,6 +656,7 @@ igemm_split_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(64u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        pdl_launch_dependents();   // (only now: see there)
     }
     for (int i = threadIdx.x; i < (a.fq2 ? 2 : 1) * FAST_NP * COLS; i += SPLIT_THREADS) {
         const int set = i / (FAST_NP * COLS), j = i - set * FAST_NP * COLS, prm = j / COLS, c = j - prm * COLS;
@@ -768,6 +768,13 @@ igemm_split_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
     }
     __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    // the columns go back before the other CTAs are waited for
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(64u) : "memory");
+    }
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     if (warp >= EPI_WARP0) {
 #pragma unroll
@@ -812,13 +819,6 @@ igemm_split_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
             const int ch = n0 + perm_real_channel(part0 + 2 * p, sa.perm_ng);
             if (m < a.m_base + a.M && ch < a.N) *(unsigned short*)((uint8_t*)a.out + (size_t)m * a.N + ch) = (unsigned short)w;
         }
-    }
-    tc_fence_before();
-    __syncthreads();
-    if (warp == 1) {
-        __syncwarp();
-        tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(64u) : "memory");
     }
 }
 

@@ -404,6 +404,10 @@ __global__ void __launch_bounds__(ROWS_GROUP * GROUPS, GROUPS == 2 ? 1 : R == 16
     }
     tc_fence_before();
     __syncthreads();
+    if (warp == 4) {        // before the other blocks are waited for (see TMEM_BYTES)
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_slot), "r"((unsigned)(S::COLUMNS * GROUPS)) : "memory");
+    }
     if (ranks > 1) cluster_sync();
     // every block of the cluster finishes a share of the outputs
     const int there = min(max(rows, 0), R);
@@ -429,10 +433,6 @@ __global__ void __launch_bounds__(ROWS_GROUP * GROUPS, GROUPS == 2 ? 1 : R == 16
         *reinterpret_cast<uint2*>(out) = make_uint2(Elem<T>::pack2(o.x * inv, o.y * inv), Elem<T>::pack2(o.z * inv, o.w * inv));
     }
     if (ranks > 1) cluster_sync();   // no block leaves while another reads its part
-    if (warp == 4) {
-        tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_slot), "r"((unsigned)(S::COLUMNS * GROUPS)) : "memory");
-    }
 }
 
 template <typename T, int D, int R, int GROUPS>

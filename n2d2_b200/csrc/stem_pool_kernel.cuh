@@ -115,7 +115,6 @@ stem_pool_tcgen05_kernel(const __grid_constant__ CUtensorMap tmX, const StemPool
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const int lane = threadIdx.x & 31;
-    pdl_launch_dependents();
     if (warp == 0) {
         for (int i = lane; i < 2 * SP_RING + 2 * SP_SLOTS + 1; i += 32)
             mbar_init(full0 + 8u * i, i >= SP_RING && i < 2 * SP_RING ? SP_ISSUERS
@@ -129,6 +128,7 @@ stem_pool_tcgen05_kernel(const __grid_constant__ CUtensorMap tmX, const StemPool
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        pdl_launch_dependents();   // (only now: see there)
     }
     tc_fence_before();
     __syncthreads();

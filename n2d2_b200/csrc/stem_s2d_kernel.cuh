@@ -135,7 +135,6 @@ stem_s2d_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const S2dArgs a
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
-    pdl_launch_dependents();
     if (a.late_layer) pdl_wait();
 
     if (threadIdx.x == 0) {
@@ -157,6 +156,7 @@ stem_s2d_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const S2dArgs a
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      ::"r"(smem_u32(tmem_slot)), "r"(a.tmem_cols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        pdl_launch_dependents();   // (only now: see there)
     }
     for (int i = threadIdx.x; i < FAST_NP * 256; i += Z_THREADS) {
         const int prm = i >> 8, c = i & 255;

@@ -17,7 +17,8 @@ static constexpr int FAST_NP = 5;             // words per channel of a fast req
 // take the SMs the earlier kernel's CTAs leave, set up barriers, TMEM, constants and weights, and only then
 // wait (pdl_wait) for the earlier kernel to complete and its memory to be visible.  Everything that reads
 // activations or writes outputs sits behind that wait, directly or through the kernel's own barriers.
-// pdl_launch_dependents, at the start of a kernel, lets the next one begin that early.
+// pdl_launch_dependents lets the next one begin that early.  It stands at the start of a kernel, or right behind its allocation of TMEM: a kernel that starts early holds its columns until the
+// one before it has ended, which must not wait for those by then, whatever other streams hold beside it.
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 // A tensor map is read through a cache of its own; fetching it ahead takes that miss (about half a microsecond) off the first load
 __device__ __forceinline__ void prefetch_tensor_map(const CUtensorMap* tm) { asm volatile("prefetch.tensormap [%0];" ::"l"(tm) : "memory"); }

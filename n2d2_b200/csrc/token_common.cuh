@@ -67,10 +67,11 @@ static inline cudaError_t launch_token(void (*kernel)(P...), dim3 grid, int thre
 }
 
 // ----------------------------------------------------------------------------- clusters
-// TMEM is handed out at run time, and a block that waits for its share while blocks that hold theirs wait for it would wait for ever.
-// Three rules keep that from happening: a block asks for at least this much shared memory for each TMEM column (the multiprocessor's
-// 228 KB over 512 columns, rounded up), so whatever blocks of these kernels share a multiprocessor, their columns fit; it allocates
-// behind griddepcontrol.wait, so it never holds columns that the kernel before it still needs; and it lets the next kernel start only then.
+// TMEM is handed out at run time, and a block that waits for its share while blocks that hold theirs wait for it would wait for ever.  Four rules keep that from happening,
+// the first two also those of a network's kernels, which may run beside these on another stream: a block lets the next kernel start only when it has its columns, so
+// none that starts early takes what the kernel before it still needs; it gives them back before it waits for another block of its cluster, so that whoever holds columns needs nobody
+// else's to finish (blocks of a pair, which share theirs, have a multiprocessor each); it asks for at least this much shared memory for each column (the multiprocessor's
+// 228 KB over 512 columns, rounded up), so blocks of these kernels that share a multiprocessor never wait for one another; and it allocates behind griddepcontrol.wait.
 static constexpr int TMEM_BYTES = 460;
 __device__ __forceinline__ unsigned cluster_rank()
 {

@@ -196,6 +196,11 @@ __global__ void __launch_bounds__(TileWarps<BYTES>::THREADS, 1) matmul_i8_tile_k
         }
     }
     tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {        // before the other blocks are waited for (see TMEM_BYTES)
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((unsigned)COLUMNS) : "memory");
+    }
     if (ranks > 1) {
         cluster_sync();
         const int columns = min(BN, p.M - t0);
@@ -216,12 +221,6 @@ __global__ void __launch_bounds__(TileWarps<BYTES>::THREADS, 1) matmul_i8_tile_k
                         Elem<T>::from_float(fmaf((float)s[e] * sa[c], p.w_scales[channel + e], p.bias ? p.bias[channel + e] : 0.0f));
         }
         cluster_sync();     // no block leaves while another reads its sums
-    } else {
-        __syncthreads();
-    }
-    if (warp == 1) {
-        tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((unsigned)COLUMNS) : "memory");
     }
 }
 
