@@ -403,7 +403,7 @@ typedef struct n2d2b_matmul {
 int n2d2b_matmul_i8(int device, const n2d2b_matmul* matmul, n2d2b_stream stream);
 
 /* A paged cache of keys and values in 8 bits, one scale for each page and head (of keys, and of
- * values), none of them negative. */
+ * values), none of them negative; where one is 0 (or up to 2^-100), so are its codes. */
 typedef struct n2d2b_kv_cache {
     int32_t nb_pages, nb_heads;
     int32_t page_tokens;       /* 16, 32, 64 or 128 */

@@ -5,7 +5,7 @@
 // values stay in registers between the maximum and the rounding.
 //
 // Four prompts of up to 4000 tokens (8 heads of 128, keys and values): 15 us, 2.7 TB/s; bound by the short life of its 4000 blocks, each a chain of lengths, page
-// number, values, reduction and store.  One token to each of 64 sequences: 7 us, that chain once, and the codes of a page rescaled where its scale
+// number, values, reduction and store.  One token to each of 64 sequences: 5 us back to back, that chain once, and the codes of a page rescaled where its scale
 // grows.  A block for several pages would have fewer of these chains, but no page of a decoding step has a neighbour to share one with.
 #include <cstdio>
 #include <cstring>

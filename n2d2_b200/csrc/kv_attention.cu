@@ -6,16 +6,16 @@
 // exponent, so that p_j = 2^(t_j - max) is at most 1 whatever the scales are and enters the second product in few bits; the softmax's sum
 // adds p_j / sV(page of j): the p_j of that sum are about 1, as the scales go from 2^-100 to 2^121 and their reciprocals fill 32 bits.
 //
-// kv_attention_rows_kernel: 8 or 16 rows (new token x query head of one key head) a tile, for few rows: bound by reading the cache.  The
+// kv_attention_rows_kernel: 4, 8 or 16 rows (new token x query head of one key head) a tile, for few rows: bound by reading the cache.  The
 // codes go into the int8 tensor cores as they lie in memory: widening them in registers took 224 integer instructions a warp for 32
 // tokens of 128, which held a kernel of that kind to 4.5 TB/s at best.  The other operand is cut into bytes instead, which costs nothing as
 // it has few columns: a query into three signed digits of a 22-bit number (on a scale of its own row), a probability into four unsigned
-// ones of a 32-bit number.  Both products are exact in 32 bits.
+// ones of a 32-bit number (2^28 for 1).  Both products are exact in 32 bits.
 //   S^T [128 tokens][3 digits x rows] = K Q^T,   O^T [head_size][4 digits x rows] = V^T P^T
 // A thread holds a token's scores for all rows, later one element of every row's output.  The tokens of a sequence are split over a cluster of
 // up to 16 blocks, whose parts are joined through distributed shared memory at the end: nothing is kept in memory between kernels.
 //
-// 48 sequences of up to 8000 tokens (8 key heads of 128, 32 query heads, bf16): 81 to 85 us, 5.7 to 6.0 TB/s; one of 65000: 33 us, 4.0 TB/s (128 of the
+// 48 sequences of up to 8000 tokens (8 key heads of 128, 32 query heads, bf16): 81 (back to back) to 85 us, 5.7 to 6.0 TB/s; one of 65000: 33 us, 4.0 TB/s (128 of the
 // multiprocessors, a cluster of 16 for each head; the blocks' beginning and end take 8 us of it); 100 tokens, heads of 64: 5.7 us a call.
 #include <cstdio>
 #include <cstring>

@@ -11,7 +11,7 @@
 // keeps its 11 bits down to 2^-19 and is off by at most 2^-30 below that, 2^-29 with the times its row's maximum moved since.  The softmax's sum is held on 2^-4 of that scale: it adds reciprocals of the values' scales
 // from 2^-121 to 2^100.
 //
-// 4096 new tokens over 8192 (32 query heads, 8 key heads of 128, bf16): 509 to 520 us, 790 to 810 TFLOP/s, 48 % of what a large matrix product reaches.  Bound by
+// 4096 new tokens over 8192 (32 query heads, 8 key heads of 128, bf16): 509 us, 810 TFLOP/s, 48 % of what a large matrix product reaches.  Bound by
 // the latency of a row's chain (scores out of TMEM, maximum, exponentials, back into TMEM) with two warps of rows to a scheduler: no pipe is more than
 // 43 % busy (tensor 43, exponentials 31, ALU 31, issue 45).  Measured and dropped: steps of 64 tokens with a second buffer of scores (540 us: products of 64
 // columns take as long as of 100), probabilities before the maximum (553), the maximum in a pass of its own (603: TMEM is read twice).

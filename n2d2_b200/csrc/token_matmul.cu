@@ -4,8 +4,8 @@
 //
 // The sums are exact in 32 bits, so any split of k gives the same bits.
 //
-// Few tokens are bound by bringing the weights (1 x 4096 x 4096: 4.3 us, 16.8 MB; 48 x 6144 x 4096: 9.2 us), many by the tensor pipe: 4096 x 4096 x 4096
-// 47 to 57 us (2.9 to 2.4 POP/s with the clock that the power limit leaves; 79 % of the pipe's cycles).
+// Few tokens are bound by bringing the weights (us a call of many, weights in L2 / in memory: 1 x 4096 x 4096 4.8 / 6.6, 48 x 6144 x 4096 9.1 / 10.4), many by
+// the tensor pipe: 4096 x 4096 x 4096 57 us (2.4 POP/s with the clock that the power limit leaves; 48 to 54 in bursts of a few ms; 79 % of the pipe's cycles).
 #include <cstdio>
 #include <cstring>
 #include "token_common.cuh"
@@ -73,7 +73,7 @@ __device__ __forceinline__ uint4 load_bytes(const int8_t* p, int valid)
 // One tile of 128 channels x BN tokens a block.  Few tiles: the blocks of a cluster take parts of k and add their 32-bit sums up through
 // distributed shared memory, each finishing a share of the tile.  Warp 0 loads, warp 1 issues the MMAs, four warps store.  BYTES: rows that TMA cannot read (not on 16
 // bytes); twelve warps, the storing ones among them, bring them through registers first: 64 bytes a thread are under way at a time (with four warps
-// 1156 x 1024 x 3277 took 112 us, with twelve 47).
+// 1156 x 1024 x 3277 took 112 us, with twelve 47, both with the operands in L2; 68 from memory).
 template <bool BYTES> struct TileWarps { static constexpr int BRINGING = BYTES ? 12 : 4, THREADS = 64 + 32 * BRINGING; };
 template <typename T, int BN, bool BYTES>
 __global__ void __launch_bounds__(TileWarps<BYTES>::THREADS, 1) matmul_i8_tile_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap a_map, const MatmulArgs p,
@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) matmul_i8_pair_kernel(const _
 // ---- a few tokens: no tiles
 // A warp takes two output channels, 512 bytes of k of both at a time, and M tokens: loads straight to registers, four products an instruction, one
 // sum over the warp at the end.  None of what a tile needs before its first and after its last byte (barriers, TMEM, a cluster's join).  1 x 4096 x
-// 4096: 4.3 us, 3.9 TB/s with launch and end; from three or four tokens on the products take longer than the bytes.
+// 4096: 3.9 us back to back with the weights in L2, 6.6 (2.5 TB/s) with them in memory; from three or four tokens on the products take longer than the bytes.
 template <typename T, int M, bool BYTES>
 __global__ void __launch_bounds__(256) matmul_i8_rows_kernel(const MatmulArgs p)
 {
@@ -493,7 +493,7 @@ template <typename T>
 static cudaError_t launch_matmul(const MatmulArgs& p, cudaStream_t s)
 {
     const bool bytes = !token_aligned(p.a, 16) || !token_aligned(p.w, 16) || p.a_stride % 16 || p.w_stride % 16;
-    // one or two tokens, up to eight where the products are few (us, tiles / without: 1 x 4096 x 4096 6.6 / 4.3, 2 x 4096 x 4096 6.6 / 4.5, 4 x 1024 x 4096
+    // one or two tokens, up to eight where the products are few (us with the weights in L2, tiles / without: 1 x 4096 x 4096 6.6 / 3.9, 2 x 4096 x 4096 6.6 / 4.5, 4 x 1024 x 4096
     // 5.4 / 4.7, 8 x 4096 x 4096 6.7 / 7.0, 4 x 8192 x 4096 8.8 / 13.8).  Unaligned rows: one token, up to four short ones (1 x 4096 x 5999 23.8 / 17.2, 4 x
     // 10000 x 511 10.5 / 6.9, 4 x 1000 x 999 6.1 / 5.3, 2 x 4096 x 2001 9.3 / 10.8, 4 x 4096 x 4001 14.5 / 24.5, 6 x 1000 x 999 6.1 / 8.1)
     if (bytes ? p.M == 1 || (p.M <= 4 && p.M * p.K <= 4000) : p.M <= 2 || (p.M <= 8 && (long long)p.M * p.N * p.K <= 1 << 25)) {

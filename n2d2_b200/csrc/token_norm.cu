@@ -8,7 +8,8 @@
 // order in which the squares are summed, and the row's sum and maximum come out of one pass and one reduction.
 //
 // Bound by memory: 7 bytes a value with a residual of 16 bits.  8192 rows of 4096 in bf16: 39 us, 5.99 TB/s (91 % of what a copy reaches); 8 rows:
-// 3.4 us, the launch, two loads one behind the other and the reduction.
+// 2.5 us back to back, the launch, two loads one behind the other and the reduction.  Rows that are not whole vectors of 16 bytes go by an element an access: 8192 of 4095
+// 122 us, 2048 of 8191 67.
 #include <cstdio>
 #include <cstring>
 #include "token_common.cuh"
