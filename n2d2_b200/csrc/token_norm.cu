@@ -94,7 +94,8 @@ __device__ __forceinline__ void block_sum_max(float& sum, unsigned& top)
     }
 }
 
-// The scale of a row h whose squares left 32 bits: their sum again, of the row times a power of two; *scale holds the step.  A function of its own and an element at a
+// The scale of a row h whose squares left 32 bits: their sum again, of the row times a power of two; *scale holds the step.  (2^75 keeps the sum below 2^121, as it was
+// below 2^-60 times the columns, and the squares of the smallest normal values at 2^-102; 2^-80 keeps 2^31 of the largest squares below 2^127.)  A function of its own and an element at a
 // time, for kernels that it takes no registers from: within them 8192 rows of 4096 took 43 to 48 us instead of 39.
 template <typename T>
 __device__ __noinline__ void scale_again(const T* h, int columns, float by, float eps, float* scale)
@@ -108,7 +109,7 @@ __device__ __noinline__ void scale_again(const T* h, int columns, float by, floa
     }
     __syncthreads();        // all threads have read what the first reduction left
     block_sum_max(sum, unused);
-    if (threadIdx.x == 0) *scale *= by * rsqrtf(sum / (float)columns + eps * by * by);
+    if (threadIdx.x == 0) *scale = (float)((double)*scale * by * rsqrtf(sum / (float)columns + eps * by * by));      // (1 / h itself may leave 32 bits)
 }
 
 // A block takes a row.  ITER > 0: a thread keeps its ITER vectors of the row in registers; ITER = 0: rows of any length, read a
@@ -210,7 +211,7 @@ __global__ void __launch_bounds__(512, ITER < 4 || VEC == 1 ? 4 : VEC == 4 ? 3 :
     }
     if (large || small) {
         if (a.residual) __syncthreads();        // (an element's sum may be another thread's)
-        scale_again<T>(a.residual ? (const T*)a.total + row * a.total_stride : (const T*)a.x + row * a.x_stride, a.columns, large ? 0x1p-80f : 0x1p60f, a.eps, a.scales + row);
+        scale_again<T>(a.residual ? (const T*)a.total + row * a.total_stride : (const T*)a.x + row * a.x_stride, a.columns, large ? 0x1p-80f : 0x1p75f, a.eps, a.scales + row);
     }
 }
 

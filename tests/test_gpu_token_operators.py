@@ -969,3 +969,14 @@ def test_a_layer_against_the_layer_in_64_bits(lengths, news):
     want = attended.flatten(1) @ (w_out.double() * w_out_scales.double()[:, None]).T
     off = (back.double() - want).square().mean().sqrt() / want.square().mean().sqrt()
     assert off <= 0.026, float(off)
+
+
+@pytest.mark.parametrize('columns', [5, 512, 4095])
+@pytest.mark.parametrize('power, lift', [(-120, 40), (-125, 60), (-100, 10), (-135, 100)])
+def test_norm_of_the_smallest_rows_under_large_weights(power, lift, columns):
+    g = gen(columns)
+    x = (1 + normal(2, columns, g=g).abs()) * 2.0 ** power
+    w = (1 + 0.3 * normal(columns, g=g)) * 2.0 ** lift
+    codes, scales = torch.zeros((2, columns), dtype=torch.int8, device='cuda'), torch.zeros(2, device='cuda')
+    runtime.rmsnorm_quantize(x.data_ptr(), 2, columns, w.data_ptr(), codes.data_ptr(), scales.data_ptr(), dtype='f32', eps=0.0)
+    check_norm(x, w, codes, scales, 'f32', 0.0)
