@@ -442,7 +442,8 @@ int n2d2b_kv_append(int device, const n2d2b_kv_cache* cache, const n2d2b_kv_batc
  * A query at position p (the last new token stands at lengths - 1) sees the tokens j < length, with `causal` only j <= p, and with a
  * `window` > 0 (causal only) only j > p - window.  One that sees nothing gives zeros.  Scores, the softmax's sums and the output's sums are
  * held in 32 bits.  The products take a query's value to within 2^-21 of the largest of its row, and a probability (weighted with the scale of its
- * page's values) to within 2^-11 of itself or 2^-29 of the largest of its row, whichever is more; the softmax's sum takes it in 32 bits. */
+ * page's values) to within 2^-11 of itself or 2^-29 of the largest of its row, whichever is more; the softmax's sum takes it in 32 bits.  Where scales of
+ * the values that a row sees lie more than 2^100 apart (a scale of 0 counts as 2^-80 there), tokens of the smaller ones may drop out of that sum. */
 typedef struct n2d2b_attention {
     int32_t dtype;             /* of q and out: N2D2B_F16 or N2D2B_BF16 */
     int32_t nb_query_heads;    /* a multiple of the cache's heads */
