@@ -407,7 +407,6 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_attention_prompt_kernel(cons
                         if (moves) top = raised;
                         sum *= fade;
                         tc_wait_st();       // what the quarters before stored: only this orders the loads behind it
-                        const __half2 fade2 = __float2half2_rn(fade);
 #pragma unroll 1
                         for (int c = 0; c < 16 * q; c += 16) {        // this block's probabilities so far
                             unsigned p[16];
@@ -416,8 +415,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_attention_prompt_kernel(cons
 #pragma unroll
                             for (int e = 0; e < 16; ++e) {
                                 asm volatile("" : "+r"(p[e])::"memory");
-                                const __half2 h = __hmul2(*reinterpret_cast<__half2*>(&p[e]), fade2);
-                                p[e] = *reinterpret_cast<const unsigned*>(&h);
+                                // (in 32 bits: factors below 2^-24 are no halves, but up to 2^14 times them are)
+                                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p[e]));
+                                p[e] = pack_half2(f.x * fade, f.y * fade);
                             }
                             tc_st16(s_at + (unsigned)c, p);
                         }

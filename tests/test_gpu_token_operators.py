@@ -980,3 +980,36 @@ def test_norm_of_the_smallest_rows_under_large_weights(power, lift, columns):
     codes, scales = torch.zeros((2, columns), dtype=torch.int8, device='cuda'), torch.zeros(2, device='cuda')
     runtime.rmsnorm_quantize(x.data_ptr(), 2, columns, w.data_ptr(), codes.data_ptr(), scales.data_ptr(), dtype='f32', eps=0.0)
     check_norm(x, w, codes, scales, 'f32', 0.0)
+
+
+@pytest.mark.parametrize('levels', [(-26, -18, 0, -26), (-25.5, -17.5, -17, 0), (-30.5, -20, -17, 0), (-18, -18, 0, -18), (-30.5, -17, -30.5, 0), (-12, -16, -4, 0), (0, -18, -16, -17)])
+@pytest.mark.parametrize('size', [64, 128])
+def test_attention_of_many_rows_keeps_what_came_before_a_maximum(size, levels):
+    """Tokens of 2^-12 to 2^-20 of a row's largest, in the quarters of a step before it: every probability by itself, as each token's values stand in an element of their own."""
+    s = Served([128] * 2, [128] * 2, 8, size, 64, 'f16', heads=128)
+    c = torch.tensor([4 * x for x in levels], device='cuda').repeat_interleave(32)       # quarters of log2, a token's score
+    c = c - 4 * torch.rand(128, device='cuda', generator=s.g).mul(2).floor().where(c < 0, torch.zeros_like(c))     # and some of one less
+    c[c == 0] = -120
+    c[32 * levels.index(0) + 11] = 0
+    s.q.copy_(s.q[:1, :1].sign())
+    s.k_scales.fill_(0.01)
+    s.v_scales.fill_(100.0)
+    s.v.zero_()
+    at = torch.arange(128, device='cuda')
+    out = []
+    for part in range(128 // size):                  # (heads of 64 have room for half of the tokens at a time)
+        s.v.zero_()
+        for row in s.table:
+            pages = torch.tensor(row[:2], device='cuda')[at // 64]
+            s.k[pages, :, at % 64] = (c[:, None] * s.q[0, 0].float()).to(torch.int8)[:, None]
+            mine = at // size == part
+            s.v[pages[mine], :, at[mine] % 64, at[mine] % size] = 127
+        out.append(s.attention(scale=0.25 * math.log(2) / (size * 0.01), causal=False)[:s.tokens].double() / 12700)
+    runtime.token_check()
+    p = torch.cat(out, 2)
+    want = 2.0 ** (c.double() / 4)
+    want = want / want.sum()
+    # scores are exact but for the 32-bit scale (2^-22 of up to 30); 2^-18 of the polynomial, 11 bits down to 2^-19, then 2^-29 of the largest; the output's rounding
+    bound = want * (30 * 2.0 ** -21 + 2.0 ** -17 + 2.0 ** -11 + half_step('f16') * 1.01) + 2.0 ** -29 + 2.0 ** -25 / 12700
+    off = (p - want).abs()
+    assert (off <= bound).all(), (float((off - bound).max()), int((off - bound).amax((0, 1)).argmax()))
