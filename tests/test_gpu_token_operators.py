@@ -1013,3 +1013,37 @@ def test_attention_of_many_rows_keeps_what_came_before_a_maximum(size, levels):
     bound = want * (30 * 2.0 ** -21 + 2.0 ** -17 + 2.0 ** -11 + half_step('f16') * 1.01) + 2.0 ** -29 + 2.0 ** -25 / 12700
     off = (p - want).abs()
     assert (off <= bound).all(), (float((off - bound).max()), int((off - bound).amax((0, 1)).argmax()))
+
+
+@pytest.mark.parametrize('window', [0, 70])
+@pytest.mark.parametrize('size, page, kv_heads, group, length, new, batch', [
+    (64, 16, 1, 4, 1000, 1, 1), (128, 64, 2, 2, 700, 4, 3), (128, 32, 2, 16, 600, 1, 12), (64, 128, 8, 8, 500, 60, 3), (128, 16, 8, 16, 400, 300, 2), (64, 64, 2, 16, 900, 300, 12)])
+def test_attention_every_probability_by_itself(size, page, kv_heads, group, length, new, batch, window):
+    """Each token's values stand in an element of their own, so that an output is its probability: to within 2^-11 of itself or 2^-29 of the row's largest, as the
+    header has it, wherever maxima move."""
+    s = Served([length] * batch, [new] * batch, kv_heads, size, page, 'f16', heads=kv_heads * group)
+    s.k_scales.mul_(2.0 ** torch.randint(-2, 3, s.k_scales.shape, device='cuda', generator=s.g))
+    s.v_scales.fill_(2.0 ** 14 / 127).mul_(2.0 ** -torch.randint(0, 4, s.v_scales.shape, device='cuda', generator=s.g))
+    scale, at, parts = size ** -0.5, torch.arange(length, device='cuda'), []
+    for lo in range(0, length, size):
+        s.v.zero_()
+        t = at[lo:lo + size]
+        for row in s.table:
+            s.v[torch.tensor(row, device='cuda')[t // page], :, t % page, t % size] = 127
+        parts.append(s.attention(scale=scale, window=window)[:s.tokens].double()[..., :len(t)] / 127)
+    runtime.token_check()
+    got = torch.cat(parts, 2)
+    position = torch.arange(length - new, length, device='cuda')[:, None]
+    seen = (at <= position) & ((at > position - window) if window else True)
+    for b in {0, batch - 1}:
+        used = torch.tensor(s.table[b][:-(-length // page)], device='cuda')
+        for h in range(0, s.heads, max(1, group - 1)):
+            sv = s.v_scales[used, h // group].double().repeat_interleave(page)[:length]
+            k = (s.k[used, h // group].double() * s.k_scales[used, h // group].double()[:, None, None]).flatten(0, 1)[:length]
+            q = s.q[b * new:(b + 1) * new, h].double()
+            p = torch.softmax((q @ k.T * scale).masked_fill(~seen, -math.inf), 1) * sv
+            # scores as in check_attention, queries to within 2^-21 of the row's largest; the output's own rounding beside the two bounds
+            delta = (q.abs() @ k.abs().T * scale).amax(1, keepdim=True) * (size + 8) * 2 * U + scale * q.abs().amax(1, keepdim=True) * k.abs().sum(1).max() * 2.0 ** -21
+            bound = p * (2 * delta + 2.0 ** -11 + half_step('f16') * 1.01 + (length / 16 + 100) * 4 * U) + 2.0 ** -29 * p.amax(1, keepdim=True) + 2.0 ** -25 / 127
+            off = (got[b * new:(b + 1) * new, h] - p).abs()
+            assert (off <= bound).all(), (b, h, float((off / bound).max()))
